@@ -372,6 +372,40 @@ int lme_ce_stats(const void* logits, long long ld, const long long* labels, floa
 // gradient scale = scale * (*scale_dev if scale_dev != NULL)
 int lme_ce_grad(void* logits, long long ld, const long long* labels, const float* lse, int T, int V, int v0,
                 float scale, const float* scale_dev, long long ignore_index, void* stream);
+// Rows of logits over a vocabulary.  dtype: LME_BF16, LME_F16 or LME_F32.  Row r of `rows` starts at
+// x + (r / inner) * ld_outer + (r % inner) * ld_inner elements and may start at any element; a gradient is dense [rows, V]
+// in the same type.  temperature > 0 divides the logits.  k <= LME_VOCAB_MAX_K.
+#define LME_BF16 0
+#define LME_F16 1
+#define LME_F32 2
+#define LME_VOCAB_MAX_K 128
+// Log probabilities of tokens [rows] (NULL: none; 0 where a token is ignore_index, NaN where it is outside of [0, V)),
+// entropies [rows], and with k > 0 the k <= V largest logits' log probabilities and places [rows, k] in order, the lowest place
+// first among equal logits.  stats (optional, 4 floats per row, 16-byte aligned) is what the gradient needs.
+int lme_token_logprobs_fwd(const void* x, int dtype, long long rows, long long inner, long long ld_inner,
+                           long long ld_outer, int V, const long long* tokens, long long ignore_index, double temperature,
+                           int k, float* logprobs, float* entropy, float* top_logprobs, long long* top_ids, float* stats,
+                           void* stream);
+// grad = gradient of the logits; d_logprobs, d_entropy [rows] and d_top [rows, k] are optional
+int lme_token_logprobs_bwd(const void* x, int dtype, long long rows, long long inner, long long ld_inner,
+                           long long ld_outer, int V, const long long* tokens, long long ignore_index, double temperature,
+                           int k, const float* stats, const long long* top_ids, const float* d_logprobs,
+                           const float* d_entropy, const float* d_top, void* grad, void* stream);
+// Divergence kl [rows] between the softmax of the rows and a teacher known by k tokens per row (top_ids, top_logprobs
+// [rows, k]): KL(teacher || rows), or with forward_kl KL(rows || teacher); tail: one more bucket for all other tokens, whose
+// probability is 1 - the listed ones' (needed by forward_kl); without it the teacher's values are renormalised.  Entries with an id
+// outside of [0, V) or a value of -inf are absent, an id's later entries too; a row without entries has kl 0.  labels / nll
+// (both or neither): cross entropy at temperature one, 0 where a label is ignore_index.  entries (int [rows, k]) and stats
+// (8 floats per row, 16-byte aligned) are what the gradient needs.
+int lme_topk_distillation_fwd(const void* x, int dtype, long long rows, long long inner, long long ld_inner,
+                              long long ld_outer, int V, const long long* top_ids, const float* top_logprobs, int k,
+                              const long long* labels, long long ignore_index, double temperature, int forward_kl, int tail,
+                              float* kl, float* nll, int* entries, float* stats, void* stream);
+// grad = gradient of the logits; d_kl and d_nll [rows] are optional
+int lme_topk_distillation_bwd(const void* x, int dtype, long long rows, long long inner, long long ld_inner,
+                              long long ld_outer, int V, const int* entries, const float* top_logprobs, int k,
+                              const long long* labels, long long ignore_index, double temperature, int forward_kl,
+                              const float* stats, const float* d_kl, const float* d_nll, void* grad, void* stream);
 // torch.optim.AdamW step on a flat fp32 shard (+ refresh of the bf16 compute copy); step counts from 1
 int lme_adamw(float* p, float* m, float* v, const void* g, int g_is_bf16, void* p_lp, long long n, float lr,
               float b1, float b2, float eps, float wd, int step, const float* gscale, void* stream);

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -53,7 +53,7 @@ def cuda_lib() -> ctypes.CDLL:
     global _cuda_lib
     if _cuda_lib is None:
         lib = _load("liblme_cuda.so", "build_cuda")
-        P, I, L, F = c_void_p, c_int, c_longlong, c_float
+        P, I, L, F, D = c_void_p, c_int, c_longlong, c_float, c_double
         sigs = {
             "lme_gemm_bf16": [P, I, L, P, I, L, P, L, I, I, I, I, P, P, L, P, L, I, P],
             "lme_gemm_fp8": [P, I, L, P, I, L, P, P, P, L, I, I, I, I, P, P, L, P, L, I, P],
@@ -125,6 +125,10 @@ def cuda_lib() -> ctypes.CDLL:
             "lme_qkv_rope": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
             "lme_ce_stats": [P, L, P, P, P, P, I, I, I, P],
             "lme_ce_grad": [P, L, P, P, I, I, I, F, P, L, P],
+            "lme_token_logprobs_fwd": [P, I, L, L, L, L, I, P, L, D, I, P, P, P, P, P, P],
+            "lme_token_logprobs_bwd": [P, I, L, L, L, L, I, P, L, D, I, P, P, P, P, P, P, P],
+            "lme_topk_distillation_fwd": [P, I, L, L, L, L, I, P, P, I, P, L, D, I, I, P, P, P, P, P],
+            "lme_topk_distillation_bwd": [P, I, L, L, L, L, I, P, P, I, P, L, D, I, P, P, P, P, P],
             "lme_adamw": [P, P, P, P, I, P, L, F, F, F, F, F, I, P, P],
             "lme_sumsq": [P, I, L, P, P, I, P],
             "lme_clip_coef": [P, F, P, P, P],

@@ -1,0 +1,164 @@
+"""Distillation from a teacher that is known by its most likely tokens, and the labels' cross entropy in the same passes.
+
+The full distributions of both models (lm_engine/model_wrapper/distillation.py:113-146) are ``[T, V]`` each; a teacher's best
+tokens (:func:`lm_engine_b200.ops.token_logprobs` with ``top_k``) can be kept or stored instead.  One kernel forward (a pass over the
+student's logits) and one backward (a pass that writes their gradient), for bf16, fp16 and fp32.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+
+from ..enums import KLDivergenceMethod
+from . import _lib
+from .logprobs import KERNEL_TYPES, MAX_TOP_K, check_logits, check_tokens, kernel_usable, logit_rows
+
+#: The teacher's mass outside of its listed tokens is one minus their sum, which the rounding of fp32 log probabilities moves by
+#: about this much: a smaller rest counts as none, and as this much where its logarithm is asked for.
+NO_TAIL = 2.0 ** -20
+
+
+class TopkDistillation(NamedTuple):
+    """Per position; ``nll`` is ``None`` without labels."""
+
+    kl_divergence: torch.Tensor
+    nll: torch.Tensor | None
+
+
+def topk_distillation_reference(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor,
+                                labels: torch.Tensor | None = None,
+                                kl_divergence_method: KLDivergenceMethod = KLDivergenceMethod.backward, tail: bool = True,
+                                temperature=1.0, ignore_index: int = -100) -> TopkDistillation:
+    V = logits.size(-1)
+    teacher = top_logprobs.detach().double()
+    there = (top_ids >= 0) & (top_ids < V) & (teacher != -torch.inf)
+    same = (top_ids[..., :, None] == top_ids[..., None, :]) & there[..., None, :]
+    there = there & ~same.tril(-1).any(-1)                      # an id's first entry counts
+    asked = there.any(-1)
+    ids = torch.where(there, top_ids, 0).long()
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    if labels is None:
+        read = asked
+    else:
+        read = asked | (labels != ignore_index)
+    x = torch.where(read[..., None], x, 0.0)                    # other rows are not looked at
+    logp = torch.log_softmax(x / temperature, -1)
+    listed = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add_(-1, ids, there.int()) > 0
+    p_rest = torch.where(listed, 0.0, logp.exp()).sum(-1).double()
+    student = torch.where(there, logp.gather(-1, ids).double(), 0.0)
+    teacher = torch.where(there, teacher, -torch.inf)
+    if not tail:
+        teacher = teacher - torch.where(asked, teacher.logsumexp(-1), 0.0)[..., None]
+    q = teacher.exp()
+    q_rest = torch.zeros_like(p_rest)
+    if tail:
+        q_rest = 1 - q.sum(-1)
+        q_rest = torch.where(q_rest < NO_TAIL, 0.0, q_rest)
+    log_rest = torch.where(p_rest > 0, p_rest, 1.0).log()
+    if kl_divergence_method == KLDivergenceMethod.backward:
+        kl = torch.where(q > 0, q * (teacher - student), 0.0).sum(-1)
+        rest = q_rest * (q_rest.clamp(min=NO_TAIL).log() - torch.where(p_rest > 0, log_rest, -torch.inf))
+        kl = kl + torch.where(q_rest > 0, rest, 0.0)
+    else:
+        finite = there & (student != -torch.inf)
+        away = torch.where(finite, student, 0.0) - torch.where(finite, teacher, 0.0)
+        kl = torch.where(finite, student.exp() * away, 0.0).sum(-1)
+        kl = kl + torch.where(p_rest > 0, p_rest * (log_rest - q_rest.clamp(min=NO_TAIL).log()), 0.0)
+    kl = torch.where(asked, kl, 0.0).to(x.dtype)
+    if labels is None:
+        return TopkDistillation(kl, None)
+    inside = (labels >= 0) & (labels < V)
+    nll = F.cross_entropy(x.reshape(-1, V), torch.where(inside, labels, 0).reshape(-1).long(),
+                          reduction="none").view(labels.shape)
+    nll = torch.where(labels == ignore_index, 0.0, torch.where(inside, nll, float("nan")))
+    return TopkDistillation(kl, nll)
+
+
+class _TopkDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index):
+        x, inner, ld_inner, ld_outer = logit_rows(logits)
+        shape, dev = logits.shape[:-1], logits.device
+        K = top_ids.size(-1)
+        kl = torch.empty(shape, dtype=torch.float32, device=dev)
+        nll = torch.empty(shape, dtype=torch.float32, device=dev) if labels is not None else None
+        entries = torch.empty((*shape, K), dtype=torch.int32, device=dev)
+        stats = torch.empty((*shape, 8), dtype=torch.float32, device=dev)
+        _lib.check(_lib.cuda_lib().lme_topk_distillation_fwd(
+            x.data_ptr(), KERNEL_TYPES[x.dtype], kl.numel(), inner, ld_inner, ld_outer, x.size(-1), top_ids.data_ptr(),
+            top_logprobs.data_ptr(), K, _lib.ptr(labels), ignore_index, temperature,
+            int(method == KLDivergenceMethod.forward), int(tail), kl.data_ptr(), _lib.ptr(nll), entries.data_ptr(),
+            stats.data_ptr(), _lib.stream_ptr()), "lme_topk_distillation_fwd")
+        _lib.count_launch()
+        ctx.save_for_backward(logits, top_ids, top_logprobs, labels, entries, stats)
+        ctx.meta = (method, tail, temperature, ignore_index)
+        ctx.set_materialize_grads(False)
+        return kl, nll
+
+    @staticmethod
+    def backward(ctx, d_kl, d_nll):
+        logits, top_ids, top_logprobs, labels, entries, stats = ctx.saved_tensors
+        method, tail, temperature, ignore_index = ctx.meta
+        nothing = (None,) * 7
+        if d_kl is None and d_nll is None:
+            return None, *nothing
+        if torch.is_grad_enabled():         # a graph of the gradients is asked for
+            x = logits.view_as(logits)
+            outs = topk_distillation_reference(x, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index)
+            outs, grads = zip(*((o, g) for o, g in zip(outs, (d_kl, d_nll)) if g is not None))
+            return *torch.autograd.grad(outs, [x], grads, create_graph=True), *nothing
+        d_kl, d_nll = (None if g is None else g.float().contiguous() for g in (d_kl, d_nll))
+        x, inner, ld_inner, ld_outer = logit_rows(logits)
+        top_logprobs, labels, entries, stats = (None if t is None else _lib.aligned(t)
+                                                for t in (top_logprobs, labels, entries, stats))
+        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _lib.check(_lib.cuda_lib().lme_topk_distillation_bwd(
+            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // x.size(-1), inner, ld_inner, ld_outer, x.size(-1),
+            entries.data_ptr(), top_logprobs.data_ptr(), entries.size(-1), _lib.ptr(labels), ignore_index, temperature,
+            int(method == KLDivergenceMethod.forward), stats.data_ptr(), _lib.ptr(d_kl), _lib.ptr(d_nll),
+            grad.data_ptr(), _lib.stream_ptr()), "lme_topk_distillation_bwd")
+        _lib.count_launch()
+        return grad, *nothing
+
+
+def topk_distillation(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor,
+                      labels: torch.Tensor | None = None,
+                      kl_divergence_method: KLDivergenceMethod | str = KLDivergenceMethod.backward, tail: bool = True,
+                      temperature: float = 1.0, ignore_index: int = -100) -> TopkDistillation:
+    """Divergence of every position between the student ``p = softmax(logits / temperature)`` over the whole vocabulary and a
+    teacher ``q`` given by ``k <= 128`` tokens per position (``top_ids``, ``top_logprobs`` ``[..., k]``, in any order).
+
+    ``kl_divergence_method``: ``backward`` = ``sum q ln(q / p)``, ``forward`` = ``sum p ln(p / q)``.  With ``tail`` the sums have one
+    more bucket, all tokens that are not listed; ``top_logprobs`` are then log probabilities at the same temperature, and the
+    teacher's rest is one minus their sum (none below 2^-20, which is also the least that ``forward`` divides by).  Without it
+    (``backward`` only) they may be logits as well, divided by the temperature, and are renormalised over the list.
+
+    An entry with an id outside of the vocabulary or a value of minus infinity is absent, an id given twice counts with its first
+    entry.  A position without entries has divergence 0 and takes no part; so padding is ids of -1.
+
+    ``labels``: the negative log likelihood of the labels at temperature one, from the same passes; 0 where a label is
+    ``ignore_index``, NaN (and no gradient) outside of the vocabulary.  Both results are fp32 (fp64 for fp64 logits) and differentiable in
+    the logits, which must hold the whole vocabulary; the teacher gets no gradient."""
+    check_logits(logits, temperature)
+    method = KLDivergenceMethod(kl_divergence_method)
+    if method == KLDivergenceMethod.forward and not tail:
+        raise ValueError("kl_divergence_method forward needs the tail: without it tokens outside of the list have no probability")
+    K = top_ids.size(-1) if top_ids.dim() else 0
+    if not 1 <= K <= MAX_TOP_K:
+        raise ValueError(f"a teacher's list has 1..{MAX_TOP_K} tokens, got top_ids of {tuple(top_ids.shape)}")
+    check_tokens("top_ids", top_ids[..., 0], logits)
+    if top_logprobs.shape != top_ids.shape or not top_logprobs.is_floating_point():
+        raise ValueError(f"top_logprobs need a floating type and shape {tuple(top_ids.shape)}, got {top_logprobs.dtype} of "
+                         f"{tuple(top_logprobs.shape)}")
+    if labels is not None:
+        check_tokens("labels", labels, logits)
+    if not kernel_usable(logits, temperature, top_ids, top_logprobs, labels):
+        return topk_distillation_reference(logits, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index)
+    if labels is not None:
+        labels = labels.to(torch.int64).contiguous()
+    return TopkDistillation(*_TopkDistillation.apply(
+        logits, top_ids.to(torch.int64).contiguous(), top_logprobs.detach().float().contiguous(), labels, method,
+        bool(tail), float(temperature), int(ignore_index)))
