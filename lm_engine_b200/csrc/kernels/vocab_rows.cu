@@ -18,9 +18,10 @@ namespace vr {
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int UNROLL = 4;               // vectors of 16 bytes per thread and step
+constexpr int WARP_STEP = 32 * UNROLL;  // vectors of a warp and step
 constexpr int MAX_SPLITS = 8;           // CTAs of a cluster
 constexpr int MAX_K = LME_VOCAB_MAX_K;  // best tokens, or tokens of a teacher, per row
-constexpr int SEGMENTS = 4;             // of a CTA's steps: the maxima that the selection starts from
+constexpr int SEGMENTS = 8;             // of a CTA's steps: what the selection reads again goes by their maxima
 constexpr int MAX_CANDIDATES = 2048;
 constexpr int MAX_MAP = 96 * 1024;      // bytes of the map of listed tokens: a byte per vector of a CTA
 constexpr float T_MIN = -150.f;         // 2^-150 is zero here; keeps 0 * (-inf) out of the sums
@@ -38,6 +39,32 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// two fp32 values per instruction: the stream is bound by its instructions about as much as by HBM
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(unsigned long long p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 template <typename T>
 struct Elem;
 template <>
@@ -45,8 +72,17 @@ struct Elem<__nv_bfloat16> {
     static constexpr int N = 8;         // per vector
     static constexpr int KEY_BITS = 16; // of an ordered key that differ between values
     static constexpr uint32_t NEG_INF = 0xff80ff80u;
+    static constexpr uint32_t LOW2 = 0xf14af14au;       // two of LOW
+    static constexpr float LOW = -1.00025555e30f;
     static __device__ __forceinline__ float f(__nv_bfloat16 x) { return __bfloat162float(x); }
-    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) { unpack8(u, f); }
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
         uint32_t r;
         asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -66,6 +102,8 @@ struct Elem<__half> {
     static constexpr int N = 8;
     static constexpr int KEY_BITS = 19; // fp16 as fp32 bits: 13 zeros at the end
     static constexpr uint32_t NEG_INF = 0xfc00fc00u;
+    static constexpr uint32_t LOW2 = 0xfbfffbffu;
+    static constexpr float LOW = -65504.f;
     static __device__ __forceinline__ float f(__half x) { return __half2float(x); }
     static __device__ __forceinline__ float2 two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
     static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
@@ -100,6 +138,8 @@ struct Elem<float> {
     static constexpr int N = 4;
     static constexpr int KEY_BITS = 20; // the selection's first bound may be coarse
     static constexpr uint32_t NEG_INF = 0xff800000u;
+    static constexpr uint32_t LOW2 = 0;
+    static constexpr float LOW = 0.f;                   // (one value per word: nothing is gained)
     static __device__ __forceinline__ float f(float x) { return x; }
     static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
         f[0] = __uint_as_float(u.x);
@@ -126,7 +166,8 @@ struct Rows {
     int V;
     template <typename T>
     __device__ __forceinline__ const T* row(long long r) const {
-        const long long o = r / inner;
+        if (r < inner) return static_cast<const T*>(x) + r * ld_inner;
+        const unsigned o = static_cast<unsigned>(r) / static_cast<unsigned>(inner);     // (at most 2^31 rows)
         return static_cast<const T*>(x) + o * ld_outer + (r - o * inner) * ld_inner;
     }
 };
@@ -155,12 +196,16 @@ struct Slice {
         full1 = end - (tail ? 1 : 0);
     }
     __device__ __forceinline__ int index(int j, int e) const { return j * N + e - before; }
+    __device__ __forceinline__ int size() const {           // values of this CTA
+        return max(0, min(V, end * N - before) - max(0, begin * N - before));
+    }
     __device__ __forceinline__ bool has(int id) const {     // whether token `id` is in this CTA's vectors
         const int j = (id + before) / N;
         return id >= 0 && id < V && j >= begin && j < end;
     }
+    __device__ __forceinline__ const T* at(int j) const { return row - before + static_cast<long long>(j) * N; }
     __device__ __forceinline__ uint4 load(int j) const {    // a whole vector
-        const T* p = row - before + static_cast<long long>(j) * N;
+        const T* p = at(j);
         uint4 r;
         asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                      : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
@@ -184,6 +229,103 @@ struct Slice {
     __device__ __forceinline__ bool whole(int j) const { return j >= full0 && j < full1; }
     __device__ __forceinline__ uint4 load_any(int j) const { return whole(j) ? load(j) : load_part(j); }
     __device__ __forceinline__ int steps() const { return (full1 - full0 + THREADS * UNROLL - 1) / (THREADS * UNROLL); }
+    // this thread's vectors of a step: j, j + 32, ...
+    __device__ __forceinline__ int first(int step) const {
+        return full0 + step * (THREADS * UNROLL) + static_cast<int>(threadIdx.x >> 5) * WARP_STEP + static_cast<int>(threadIdx.x & 31);
+    }
+};
+
+// A warp's whole vectors arrive in a ring of its own, `stages` steps of 2 KB that one lane requests ahead: the loads in
+// flight take no registers, and no warp waits for another.
+template <typename T>
+struct Ring {
+    static constexpr uint32_t BYTES = WARP_STEP * 16;
+    uint32_t buf, full;     // shared addresses of this warp's stages and barriers
+    const T* source;        // of the next request
+    int stages, steps;      // steps: those in which this warp has vectors
+    int last;               // vectors of the last one
+    int ahead;              // requests so far
+    bool ok;
+
+    __device__ __forceinline__ Ring(const Slice<T>& sl, uint8_t* smem, int stages_) : stages(stages_), ahead(0), ok(true) {
+        const int warp = threadIdx.x >> 5;
+        buf = smem_u32(smem) + warp * stages * BYTES;
+        uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * stages * BYTES) + warp * stages;
+        full = smem_u32(bars);
+        const int j = sl.full0 + warp * WARP_STEP;
+        steps = j < sl.full1 ? (sl.full1 - j - 1) / (THREADS * UNROLL) + 1 : 0;
+        last = min(WARP_STEP, sl.full1 - j - (steps - 1) * (THREADS * UNROLL));
+        source = sl.at(j);
+        if ((threadIdx.x & 31) == 0) {
+            for (int i = 0; i < stages; ++i) mbar_init(bars + i, 1);
+            fence_barrier_init();
+            for (int i = 0; i < stages; ++i) request(i);
+        }
+        __syncwarp();
+    }
+    // one lane: the next step into a slot, if there is one
+    __device__ __forceinline__ void request(int slot) {
+        if (ahead >= steps) return;
+        const uint32_t bytes = ++ahead == steps ? last * 16 : BYTES;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * slot), "r"(bytes) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(buf + slot * BYTES),
+                     "l"(source), "r"(bytes), "r"(full + 8 * slot)
+                     : "memory");
+        source += THREADS * UNROLL * Elem<T>::N;
+    }
+    static __device__ __forceinline__ uint4 ld(uint32_t address) {
+        uint4 r;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(address) : "memory");
+        return r;
+    }
+    // f(step, vectors, whether all of them are there) for every step; nothing behind the last whole vector.  After a wait that ran out the loop goes on
+    // without waiting (wrong rows, status word set).
+    // first(step, address): before a lane reads its vectors, 512 bytes apart from `address` on.
+    template <typename F0, typename F>
+    __device__ __forceinline__ void stream(F0&& first, F&& f) {
+        const int lane = threadIdx.x & 31;
+        for (int step = 0, slot = 0, phase = 0; step < steps; ++step) {
+            if (ok) ok = wait(full + 8 * slot, phase);
+            const uint32_t b = buf + slot * BYTES + lane * 16;
+            first(step, b);
+            uint4 v[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) v[u] = ld(b + 512 * u);
+            const bool whole = step < steps - 1 || last == WARP_STEP;
+            if (!whole)
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u)
+                    if (lane + 32 * u >= last) v[u] = Slice<T>::nothing();      // (and not what the slot held)
+            f(step, v, whole);
+            // Only now: what a lane has used it has read.  (Requested right behind the reads, a stage was overwritten under them.)
+            __syncwarp();
+            if (lane == 0) request(slot);
+            if (++slot == stages) {
+                slot = 0;
+                phase ^= 1;
+            }
+        }
+    }
+    // waits for what has been requested and not used: no copy may outlast its CTA
+    __device__ __forceinline__ void drain() {
+        for (int i = 0; i < min(stages, steps); ++i) wait(full + 8 * i, 0);
+    }
+
+private:
+    static __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+        uint32_t there;
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t"
+            "}\n"
+            : "=r"(there)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (there) return true;
+        return mbar_wait(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity, 620);
+    }
 };
 
 template <typename T, int U>
@@ -199,11 +341,29 @@ __device__ __forceinline__ float max_of(const uint4 (&r)[U]) {
     return Elem<T>::max_halves(w);
 }
 
+__host__ __device__ constexpr int ring_bytes(int stages) { return WARPS * stages * (WARP_STEP * 16 + 8); }
+
 // ------------------------------------------------------------------ running sums of a thread
-// m: largest logit so far, s: sum of 2^t, w: sum of 2^t t with t = (x - m) c.  A NaN reaches all three.
-template <bool ENTROPY, bool TWO>
+// m: a base that no logit so far is above by more than SLACK / c, s: sum of 2^t, w: sum of 2^t t with t = (x - m) c.  The base
+// follows the largest logit only past the slack: a thread meets a new largest in most of its steps at first, and its warp with
+// it, but few that are so much larger.  A NaN reaches all three.
+//
+// That is nine instructions per logit, and sustained the power limit makes each of them cost time.  So after a first step
+// that sets the base, steps are tried in three and a half: t = x c - n in one rounding, n an integer next to m c (units of 2^n
+// until leave()), no largest logit and no guard for minus infinity, and the sums are looked at afterwards; where they have run
+// over or are NaN the step is done again in the careful way, and the rest of the row too.
+constexpr float SLACK = 8.f;
+constexpr float TRY_BELOW = 1.2676506e30f;              // 2^100
+// AT_ONE: how the sum at temperature one is found beside the other: not at all, by exponentials of its own (as many again, and the
+// exponential unit is what bounds the stream then), or at temperature two by squares.  Distillation of 4096 x 128256
+// bf16 logits at temperature two, forward: 277 us with exponentials of their own, 205 with squares.
+enum AtOne { NONE, OWN, SQUARE };
+template <bool ENTROPY, AtOne ONE>
 struct Running {
-    float m = -INFINITY, s = 0.f, w = 0.f, s1 = 0.f;    // s1: s at temperature one (c1)
+    float m = -INFINITY, limit = -INFINITY, s = 0.f, w = 0.f, s1 = 0.f;    // s1: s at temperature one (c1)
+    bool far = false;               // LOW is so far below the base that it counts nothing
+    bool trying = false, tried = false;
+    float n = 0.f, n1 = 0.f;        // while trying
 
     __device__ __forceinline__ void raise(float to, float c, float c1) {
         const float d = m - to;
@@ -211,37 +371,105 @@ struct Running {
         const float f = exp2_approx(t);
         if (ENTROPY) w = (w + s * t) * f;
         s *= f;
-        if (TWO) s1 *= exp2_approx(max_nan(d * c1, T_MIN));
+        if (ONE) s1 *= exp2_approx(max_nan(d * c1, T_MIN));
         m = to;
+        limit = to + __fdividef(SLACK, ONE ? fmaxf(c, c1) : c);
     }
-    template <typename T, int U>
-    __device__ __forceinline__ void add(const uint4 (&r)[U], float largest, float c, float c1) {
+    // from units of 2^(m c) to those of 2^n and back
+    __device__ __forceinline__ void change(float by, float by1) {
+        const float f = exp2_approx(by);
+        if (ENTROPY) w = (w + s * by) * f;
+        s *= f;
+        if (ONE == SQUARE) s1 *= f * f;
+        if (ONE == OWN) s1 *= exp2_approx(by1);
+    }
+    __device__ __forceinline__ void enter(float c, float c1) {
+        if (m == -INFINITY) return;                     // (no base yet)
+        tried = true;
+        if (!(fabsf(m) * (ONE == OWN ? fmaxf(c, c1) : c) < 1e6f)) return;
+        n = rintf(m * c);
+        n1 = ONE == OWN ? rintf(m * c1) : 0.f;
+        change(fmaf(m, c, -n), fmaf(m, c1, -n1));
+        trying = true;
+    }
+    __device__ __forceinline__ void leave(float c, float c1) {
+        if (!trying) return;
+        change(-fmaf(m, c, -n), -fmaf(m, c1, -n1));
+        trying = false;
+    }
+    // whole: no vector of the step is filled up; largest(): of the step
+    template <typename T, int U, typename F>
+    __device__ __forceinline__ void add(const uint4 (&r)[U], bool whole, F&& largest, float c, float c1) {
+        if (trying) {
+            if (whole) {
+                const float s_ = s, w_ = w, s1_ = s1;
+                sum<T, U, true, false, false>(r, c, c1);
+                if (s < TRY_BELOW && (!ENTROPY || fabsf(w) < INFINITY) && (!ONE || s1 < TRY_BELOW)) return;
+                s = s_;
+                w = w_;
+                s1 = s1_;
+            }
+            leave(c, c1);
+        }
+        const float x = largest();
+        if (!(x <= limit)) {
+            raise(x, c, c1);
+            far = m - Elem<T>::LOW > __fdividef(200.f, c) && c < 1e8f;
+        }
+        // 0 * (-inf) must not get into w: a limit on t costs an instruction per logit, one on the packed logits half of one, and
+        // serves where what it turns a logit into is zero too
+        if (!ENTROPY) sum<T, U, false, false, false>(r, c, c1);
+        else if (Elem<T>::N == 8 && far) sum<T, U, false, true, false>(r, c, c1);
+        else sum<T, U, false, false, true>(r, c, c1);
+        if (!tried) enter(c, c1);
+    }
+    template <typename T, int U, bool TRY, bool LIMIT_X, bool LIMIT_T>
+    __device__ __forceinline__ void sum(const uint4 (&r)[U], float c, float c1) {
         constexpr int N = Elem<T>::N;
-        if (!(largest <= m)) raise(largest, c, c1);
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = TRY ? n : m == -INFINITY ? 0.f : m;
+        const unsigned long long nb = pair(-base, -base), nb1 = pair(-n1, -n1), cc = pair(c, c), cc1 = pair(c1, c1);
+        unsigned long long s2 = pair(s, 0.f), w2 = pair(w, 0.f), s12 = pair(s1, 0.f);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            uint4 v = r[u];
+            if (LIMIT_X) {
+                constexpr uint32_t low = Elem<T>::LOW2;
+                v = make_uint4(Elem<T>::max2(v.x, low), Elem<T>::max2(v.y, low), Elem<T>::max2(v.z, low), Elem<T>::max2(v.w, low));
+            }
             float f[N];
-            Elem<T>::unpack(r[u], f);
+            Elem<T>::unpack(v, f);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float d = f[e] - base;
-                const float t = max_nan(d * c, T_MIN);
-                const float p = exp2_approx(t);
-                s += p;
-                if (ENTROPY) w = fmaf(p, t, w);
-                if (TWO) s1 += exp2_approx(max_nan(d * c1, T_MIN));
+            for (int e = 0; e < N; e += 2) {
+                const unsigned long long x = pair(f[e], f[e + 1]), d = TRY ? x : add2(x, nb);
+                float2 t = halves(TRY ? fma2(x, cc, nb) : mul2(d, cc));
+                if (LIMIT_T) {
+                    t.x = max_nan(t.x, T_MIN);
+                    t.y = max_nan(t.y, T_MIN);
+                }
+                const unsigned long long q = pair(exp2_approx(t.x), exp2_approx(t.y));
+                s2 = add2(s2, q);
+                if (ENTROPY) w2 = fma2(q, pair(t.x, t.y), w2);
+                if (ONE == SQUARE) s12 = fma2(q, q, s12);
+                if (ONE == OWN) {
+                    const float2 t1 = halves(TRY ? fma2(x, cc1, nb1) : mul2(d, cc1));
+                    s12 = add2(s12, pair(exp2_approx(t1.x), exp2_approx(t1.y)));
+                }
             }
         }
+        const float2 a = halves(s2), b = halves(w2), a1 = halves(s12);
+        s = a.x + a.y;
+        if (ENTROPY) w = b.x + b.y;
+        if (ONE) s1 = a1.x + a1.y;
     }
 };
-// The CTA's sums, relative to its largest logit, in every thread (`red`: 4 * WARPS floats).
+// The CTA's sums, relative to its largest base, in every thread (`red`: 4 * WARPS floats).
 struct Sums {
     float m;
     double s, w, s1;
 };
-template <bool ENTROPY, bool TWO>
-__device__ __forceinline__ Sums join_block(Running<ENTROPY, TWO> r, float c, float c1, float* red) {
+template <bool ENTROPY, AtOne ONE>
+__device__ __forceinline__ Sums join_block(Running<ENTROPY, ONE> r, float c, float c1, float* red) {
+    r.leave(c, c1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float m = r.m;
 #pragma unroll
@@ -251,7 +479,7 @@ __device__ __forceinline__ Sums join_block(Running<ENTROPY, TWO> r, float c, flo
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) m = max_nan(m, red[i]);
     if (!(m <= r.m)) r.raise(m, c, c1);
-    const float s = warp_sum(r.s), w = ENTROPY ? warp_sum(r.w) : 0.f, s1 = TWO ? warp_sum(r.s1) : 0.f;
+    const float s = warp_sum(r.s), w = ENTROPY ? warp_sum(r.w) : 0.f, s1 = ONE ? warp_sum(r.s1) : 0.f;
     if (lane == 0) {
         red[WARPS + warp] = s;
         red[2 * WARPS + warp] = w;
@@ -263,7 +491,7 @@ __device__ __forceinline__ Sums join_block(Running<ENTROPY, TWO> r, float c, flo
     for (int i = 0; i < WARPS; ++i) {
         t.s += red[WARPS + i];
         if (ENTROPY) t.w += red[2 * WARPS + i];
-        if (TWO) t.s1 += red[3 * WARPS + i];
+        if (ONE) t.s1 += red[3 * WARPS + i];
     }
     return t;
 }
@@ -304,25 +532,30 @@ __device__ __forceinline__ unsigned long long candidate(uint32_t key, int index)
 }
 __device__ __forceinline__ int index_of(unsigned long long c) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(c)); }
 
+constexpr int BINS = 256;
 struct Selection {
-    uint32_t group[(SEGMENTS + 1) * THREADS];           // key of the largest value of a thread's share of a segment
-    unsigned short chosen[(SEGMENTS + 1) * THREADS];
     unsigned long long cand[MAX_CANDIDATES];
     unsigned long long best[MAX_K];
-    uint32_t threshold;
+    uint4 stash[4][THREADS];                // vectors that a thread has read again
+    unsigned short chosen[(SEGMENTS + 1) * THREADS];
+    int bin[BINS];
+    uint32_t hi[WARPS], lo[WARPS];
+    float reach;
     int groups, count, scan[WARPS];
 };
 
 // The first k of the n candidates, in order, into `best`; returns how many there are.  All threads.
 __device__ __noinline__ int order_candidates(Selection& sel, int n, int k) {
     const int tid = threadIdx.x;
-    if (n <= THREADS) {                                 // everybody counts those ahead of its own
-        if (tid < n) {
-            const unsigned long long mine = sel.cand[tid];
-            int ahead = 0;
-            for (int i = 0; i < n; ++i) ahead += sel.cand[i] > mine;
-            if (ahead < k) sel.best[ahead] = mine;
-        }
+    if (n <= THREADS) {             // the place of a candidate is the number of those ahead of it: some lanes count for each
+        const int lanes = n <= THREADS / 8 ? 8 : n <= THREADS / 4 ? 4 : n <= THREADS / 2 ? 2 : 1;
+        const int at = tid / lanes, part = tid % lanes;
+        const unsigned long long mine = at < n ? sel.cand[at] : 0;
+        int ahead = 0;
+#pragma unroll 4
+        for (int i = part; i < n; i += lanes) ahead += sel.cand[i] > mine;
+        for (int o = 1; o < lanes; o *= 2) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+        if (part == 0 && at < n && ahead < k) sel.best[ahead] = mine;
     } else {
         int size = 2 * THREADS;
         while (size < n) size *= 2;
@@ -432,59 +665,115 @@ __device__ __noinline__ int select_by_passes(Selection& sel, const Slice<T>& sl,
     return min(have, k);
 }
 
-// The k best of a slice, in order, into sel.best; returns how many the slice has.  The stream has left the largest value
-// of every group (a thread's vectors of one segment).  At least k values reach the k-th largest of these, and hardly more
-// do, so only the groups that reach it are read again: 1.03 k of them where values come in no order.
-template <typename T>
-__device__ __noinline__ int select_best(Selection& sel, const Slice<T>& sl, int k, int segment_steps) {
-    constexpr int N = Elem<T>::N, GROUPS = (SEGMENTS + 1) * THREADS, PER_LANE = GROUPS / 32;
-    const int tid = threadIdx.x;
+// A value that at least k of the threads' largest values reach and hardly more do, into sel.reach: the edge of the bin of a
+// histogram in which the k-th falls.  NaN, which compares as reached, where there is no such value or the histogram finds none.
+__device__ __forceinline__ void find_reach(Selection& sel, float largest, int k) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool finite = largest > -INFINITY;            // (no vectors, or nothing but -inf: not counted)
+    const uint32_t key = key_of(largest);
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, key), lo = __reduce_min_sync(0xffffffffu, finite ? key : 0xffffffffu);
+    if (lane == 0) {
+        sel.hi[warp] = hi;
+        sel.lo[warp] = lo;
+    }
+    for (int i = tid; i < BINS; i += THREADS) sel.bin[i] = 0;
     __syncthreads();
-    if (tid < 32) {
-        uint32_t g[PER_LANE], bound = 0;
+    uint32_t top = 0, bottom = 0xffffffffu;
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) g[i] = sel.group[tid + 32 * i];
-        for (int bit = 31; bit >= 32 - Elem<T>::KEY_BITS; --bit) {
-            const uint32_t trial = bound | 1u << bit;
-            int n = 0;
+    for (int i = 0; i < WARPS; ++i) {
+        top = max(top, sel.hi[i]);
+        bottom = min(bottom, sel.lo[i]);
+    }
+    const float from = value_of(bottom), scale = __fdividef(BINS - 0.01f, value_of(top) - from);    // (0 or NaN: one bin)
+    if (finite) atomicAdd(&sel.bin[min(BINS - 1, max(0, static_cast<int>((largest - from) * scale)))], 1);
+    __syncthreads();
+    if (warp == 0) {
+        constexpr int PER = BINS / 32;
+        int n[PER], mine = 0;                           // lane 0 has the uppermost bins
 #pragma unroll
-            for (int i = 0; i < PER_LANE; ++i) n += g[i] >= trial;
-            n = __reduce_add_sync(0xffffffffu, n);
-            if (n >= k) bound = trial;
-            if (n == k) break;
+        for (int i = 0; i < PER; ++i) mine += n[i] = sel.bin[BINS - 1 - (lane * PER + i)];
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int above = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += above;
         }
-        if (tid == 0) {
-            sel.threshold = max(bound, 1u);             // 0: groups without values
-            sel.groups = sel.count = 0;
+        const uint32_t enough = __ballot_sync(0xffffffffu, upto >= k);
+        if (enough == 0) {
+            if (lane == 0) sel.reach = __int_as_float(0x7fffffff);
+        } else if (lane == __ffs(enough) - 1) {
+            int b = BINS - 1 - lane * PER, have = upto - mine;
+#pragma unroll
+            for (int i = 0; i < PER - 1; ++i) {
+                have += n[i];
+                if (have < k) --b;
+                else have = k;
+            }
+            // below the bin's edge by more than the roundings of where its values are
+            sel.reach = from + static_cast<float>(b) / scale - (fabsf(from) + fabsf(value_of(top))) * 2e-6f;
         }
+        if (lane == 0) sel.groups = sel.count = 0;
     }
     __syncthreads();
-    const uint32_t bound = sel.threshold;
+}
+
+// The k best of a slice, in order, into sel.best; returns how many the slice has.  The stream has left each thread's largest
+// value and those of its segments (`group`).  What reaches the k-th largest of the threads' values are k values at least and
+// hardly more (1.2 k for k = 64 where values come in no order), so only the segments that do are read again.  Few
+// instructions matter more than few reads: the other CTAs of the SM stream meanwhile, and a warp gets every eighth slot.
+template <typename T>
+__device__ __noinline__ int select_best(Selection& sel, const float* group, const Slice<T>& sl, int k, float largest, int segment_steps) {
+    constexpr int N = Elem<T>::N, AHEAD = 4;
+    const int tid = threadIdx.x;
+    find_reach(sel, largest, k);
+    const float reach = sel.reach;
+    if (!(largest < reach)) {
+        uint32_t mask = 0;
 #pragma unroll
-    for (int i = 0; i < SEGMENTS + 1; ++i)
-        if (sel.group[i * THREADS + tid] >= bound) sel.chosen[atomicAdd(&sel.groups, 1)] = static_cast<unsigned short>(i * THREADS + tid);
+        for (int i = 0; i < SEGMENTS + 1; ++i) mask |= (group[i * THREADS + tid] < reach ? 0u : 1u) << i;
+        for (int at = atomicAdd(&sel.groups, __popc(mask)); mask != 0; mask &= mask - 1)
+            sel.chosen[at++] = static_cast<unsigned short>((__ffs(mask) - 1) * THREADS + tid);
+    }
     __syncthreads();
-    const int per = segment_steps * UNROLL, items = sel.groups * max(per, 1);
-    for (int i = tid; i < items; i += THREADS) {
-        const int group = sel.chosen[i / max(per, 1)], q = i - i / max(per, 1) * max(per, 1);
-        const int segment = group / THREADS, t = group - segment * THREADS;
-        int j;
-        if (segment == SEGMENTS) {                      // the parts at the row's ends
-            if (q > 0) continue;
-            j = t == 0 ? 0 : sl.nv - 1;
-        } else {
-            j = sl.full0 + (segment * per + q) * THREADS + t;
-            if (j >= sl.full1) continue;
-        }
-        float f[N];
-        Elem<T>::unpack(sl.load_any(j), f);
+    const int per = max(segment_steps, 1) * UNROLL, items = sel.groups * per;
+    for (int i0 = tid; i0 < items; i0 += AHEAD * THREADS) {
+        uint4 v[AHEAD];
+        int at[AHEAD];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint32_t key = key_of(f[e]);
-            const int v = sl.index(j, e);
-            if (key >= bound && v >= 0 && v < sl.V) {
-                const int at = atomicAdd(&sel.count, 1);
-                if (at < MAX_CANDIDATES) sel.cand[at] = candidate(key, v);
+        for (int a = 0; a < AHEAD; ++a) {
+            const int i = i0 + a * THREADS;
+            at[a] = -1;
+            if (i >= items) continue;
+            const int chosen = sel.chosen[i / per], q = i % per, segment = chosen / THREADS, t = chosen % THREADS;
+            if (segment == SEGMENTS) {                  // the parts at the row's ends
+                if (q == 0 && t == 0 && sl.head) at[a] = 0;
+                if (q == 0 && t == 1 && sl.tail) at[a] = sl.nv - 1;
+            } else {
+                const int j = sl.full0 + (segment * segment_steps + q / UNROLL) * (THREADS * UNROLL) + (t >> 5) * WARP_STEP +
+                              q % UNROLL * 32 + (t & 31);
+                if (j < sl.full1) at[a] = j;
+            }
+            if (at[a] >= 0) v[a] = sl.load_any(at[a]);
+        }
+        uint32_t hits = 0;
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (at[a] < 0) continue;
+            float f[N];
+            Elem<T>::unpack(v[a], f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) hits |= (f[e] < reach ? 0u : 1u) << (N * a + e);
+        }
+        if (hits != 0) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) sel.stash[a][tid] = v[a];
+            int to = atomicAdd(&sel.count, __popc(hits));
+            for (; hits != 0; hits &= hits - 1) {
+                const int b = __ffs(hits) - 1, a = b / N;
+                const int id = sl.index(a == 0 ? at[0] : a == 1 ? at[1] : a == 2 ? at[2] : at[3], b % N);
+                const float x = Elem<T>::f(reinterpret_cast<const T*>(&sel.stash[a][tid])[b % N]);
+                if (to < MAX_CANDIDATES) sel.cand[to] = id >= 0 && id < sl.V ? candidate(key_of(x), id) : 0ull;    // (0: a part's
+                ++to;                                                                                              // other places)
             }
         }
     }
@@ -492,7 +781,7 @@ __device__ __noinline__ int select_best(Selection& sel, const Slice<T>& sl, int 
     int n = sel.count;
     if (n > MAX_CANDIDATES) n = select_by_passes<T>(sel, sl, k);
     __syncthreads();
-    return order_candidates(sel, n, k);
+    return min(order_candidates(sel, n, k), sl.size());
 }
 
 // ------------------------------------------------------------------ log probabilities, entropies, alternatives
@@ -501,60 +790,88 @@ struct ScoreArgs {
     const long long* tokens;        // or null
     long long ignore_index;
     double inv_temperature;
-    int k, splits;
+    int k, splits, stages;
     float *logprobs, *entropy, *top_logprobs;
     long long* top_ids;
     float* stats;                   // [rows][4]: m, S, entropy, log S; or null
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const __grid_constant__ ScoreArgs p) {
+__global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid_constant__ ScoreArgs p) {
     __shared__ float red[4 * WARPS];
     __shared__ float part_m;
     __shared__ double part_s, part_w, row_log_s;
     __shared__ int part_n;
-    __shared__ std::conditional_t<TOP, Selection, int> sel;
+    extern __shared__ __align__(128) uint8_t vocab_smem[];      // the ring, and once it is empty the selection
+    __shared__ float group_[TOP ? (SEGMENTS + 1) * THREADS : 1];
+    Selection& sel = *reinterpret_cast<Selection*>(vocab_smem);
+    float* group = group_;
     const int tid = threadIdx.x;
-    const long long r = blockIdx.x / p.splits;
-    const int rank = blockIdx.x - static_cast<int>(r * p.splits);
+    const long long r = blockIdx.x / static_cast<unsigned>(p.splits);
+    const int rank = blockIdx.x % static_cast<unsigned>(p.splits);
     const T* row = p.rows.row<T>(r);
     const Slice<T> sl(row, p.rows.V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
 
-    Running<true, false> run;
+    Ring<T> ring(sl, vocab_smem, p.stages);
+    long long tok = 0;              // of the thread that finishes the row
+    float x_tok = 0.f;
+    if (p.tokens != nullptr && rank == 0 && tid == THREADS - 1) {
+        tok = p.tokens[r];
+        if (tok >= 0 && tok < p.rows.V) x_tok = Elem<T>::f(row[tok]);
+    }
+    Running<true, NONE> run;
     const int steps = sl.steps(), segment_steps = (steps + SEGMENTS - 1) / SEGMENTS;
     if constexpr (TOP)
-        for (int i = 0; i < SEGMENTS + 1; ++i) sel.group[i * THREADS + tid] = 0;
+        for (int i = 0; i < SEGMENTS + 1; ++i) group[i * THREADS + tid] = -INFINITY;
     float largest = -INFINITY;          // of the segment
-    bool some = false;
-    for (int step = 0, left = segment_steps, segment = 0; step < steps; ++step) {
-        uint4 v[UNROLL];
-        const int j0 = sl.full0 + step * THREADS * UNROLL + tid;
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) v[u] = j0 + u * THREADS < sl.full1 ? sl.load(j0 + u * THREADS) : Slice<T>::nothing();
-        const float m = max_of<T>(v);
-        run.template add<T>(v, m, c, 0.f);
-        if constexpr (TOP) {
+    float mine = -INFINITY;             // this thread's
+    int left = segment_steps, segment = 0;
+    ring.stream([](int, uint32_t) {}, [&](int step, uint4 (&v)[UNROLL], bool whole) {
+        if constexpr (!TOP) {
+            run.template add<T>(v, whole, [&] { return max_of<T>(v); }, c, 0.f);
+        } else {
+            const float m = max_of<T>(v);
+            run.template add<T>(v, whole, [&] { return m; }, c, 0.f);
             largest = max_nan(largest, m);
-            some |= j0 < sl.full1;
-            if (--left == 0 || step == steps - 1) {
-                if (some) sel.group[segment * THREADS + tid] = key_of(largest);
+            if (--left == 0 || step == ring.steps - 1) {
+                group[segment * THREADS + tid] = largest;
+                mine = max_nan(mine, largest);
                 ++segment;
                 left = segment_steps;
                 largest = -INFINITY;
-                some = false;
             }
         }
-    }
+    });
     if ((tid == 0 && sl.head) || (tid == 1 && sl.tail)) {
         const uint4 v[1] = {sl.load_part(tid == 0 ? 0 : sl.nv - 1)};
         const float m = max_of<T>(v);
-        run.template add<T>(v, m, c, 0.f);
-        if constexpr (TOP) sel.group[SEGMENTS * THREADS + tid] = key_of(m);
+        run.template add<T>(v, false, [&] { return m; }, c, 0.f);
+        if constexpr (TOP) {
+            group[SEGMENTS * THREADS + tid] = m;
+            mine = max_nan(mine, m);
+        }
     }
     Sums sum = join_block(run, c, 0.f, red);
+    // the row's last values: one thread of the last warp, while the others select
+    auto finish = [&] {
+        const double log_s = log(sum.s), entropy = log_s - sum.w / sum.s * LN2;
+        if (p.tokens != nullptr) {
+            float lp = 0.f;
+            if (tok != p.ignore_index)
+                lp = tok >= 0 && tok < p.rows.V ? static_cast<float>(static_cast<double>(x_tok - sum.m) * p.inv_temperature - log_s)
+                                                : __int_as_float(0x7fffffff);
+            p.logprobs[r] = lp;
+        }
+        p.entropy[r] = static_cast<float>(entropy);
+        if (p.stats != nullptr)
+            *reinterpret_cast<float4*>(p.stats + 4 * r) = make_float4(sum.m, static_cast<float>(sum.s), static_cast<float>(entropy),
+                                                                     static_cast<float>(log_s));
+        row_log_s = log_s;
+    };
+    if (p.splits == 1 && tid == THREADS - 1) finish();
     int n = 0;
-    if constexpr (TOP) n = select_best<T>(sel, sl, p.k, segment_steps);
+    if constexpr (TOP) n = select_best<T>(sel, group, sl, p.k, mine, segment_steps);
 
     if (p.splits > 1) {
         if (tid == 0) {
@@ -565,49 +882,41 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const __grid
         }
         cluster_sync();
         if (rank == 0) {
-            float m = sum.m;
-            for (int q = 0; q < p.splits; ++q) m = max_nan(m, ld_peer(&part_m, q));
-            double s = 0, w = 0;
-            for (int q = 0; q < p.splits; ++q) {
-                const float mq = ld_peer(&part_m, q);
-                const double t = mq == m ? 0.0 : fmax(static_cast<double>(mq - m) * c, -1000.0), f = exp2(t);
-                const double sq = ld_peer(&part_s, q);
-                s += sq * f;
-                w += (ld_peer(&part_w, q) + sq * t) * f;
+            // every warp joins the parts, a lane for each
+            const int lane = tid & 31;
+            const bool there = lane < p.splits;
+            const float mq = there ? ld_peer(&part_m, lane) : -INFINITY;
+            const int nq = there ? ld_peer(&part_n, lane) : 0;
+            double s = there ? ld_peer(&part_s, lane) : 0.0, w = there ? ld_peer(&part_w, lane) : 0.0;
+            float m = mq;
+#pragma unroll
+            for (int o = MAX_SPLITS / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            m = __shfl_sync(0xffffffffu, m, 0);
+            const float t = mq == m ? 0.f : max_nan((mq - m) * c, T_MIN), f = there ? exp2f(t) : 0.f;
+            w = (w + s * t) * f;
+            s = s * f;
+#pragma unroll
+            for (int o = MAX_SPLITS / 2; o > 0; o >>= 1) {
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+                w += __shfl_xor_sync(0xffffffffu, w, o);
             }
-            sum = Sums{m, s, w, 0.0};
+            sum = Sums{m, __shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, w, 0), 0.0};
+            if (tid == THREADS - 1) finish();
             if constexpr (TOP) {
                 int base = 0;
                 __syncthreads();
                 for (int q = 0; q < p.splits; ++q) {
-                    const int nq = ld_peer(&part_n, q);
-                    for (int i = tid; i < nq; i += THREADS) sel.cand[base + i] = ld_peer(&sel.best[i], q);
-                    base += nq;
+                    const int nb = __shfl_sync(0xffffffffu, nq, q);
+                    for (int i = tid; i < nb; i += THREADS) sel.cand[base + i] = ld_peer(&sel.best[i], q);
+                    base += nb;
                 }
                 __syncthreads();
                 n = order_candidates(sel, base, p.k);
             }
         }
     }
-    if (rank == 0) {
-        if (tid == 0) {
-            const double log_s = log(sum.s), entropy = log_s - sum.w / sum.s * LN2;
-            if (p.tokens != nullptr) {
-                const long long tok = p.tokens[r];
-                float lp = 0.f;
-                if (tok != p.ignore_index)
-                    lp = tok >= 0 && tok < p.rows.V
-                             ? static_cast<float>(static_cast<double>(Elem<T>::f(row[tok]) - sum.m) * p.inv_temperature - log_s)
-                             : __int_as_float(0x7fffffff);
-                p.logprobs[r] = lp;
-            }
-            p.entropy[r] = static_cast<float>(entropy);
-            if (p.stats != nullptr)
-                *reinterpret_cast<float4*>(p.stats + 4 * r) = make_float4(
-                    sum.m, static_cast<float>(sum.s), static_cast<float>(entropy), static_cast<float>(log_s));
-            row_log_s = log_s;
-        }
-        if constexpr (TOP) {
+    if constexpr (TOP) {
+        if (rank == 0) {
             __syncthreads();
             if (tid < n) {
                 const unsigned long long b = sel.best[tid];
@@ -622,79 +931,109 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const __grid
 
 // ------------------------------------------------------------------ gradients
 // dx_j = coefficient of the row times the row's exponentials, and other values at single tokens, which overwrite what the
-// stream has stored once the CTA has passed a barrier.  A CTA takes one step's vectors of one row: nothing depends on the
-// other CTAs, and the loads of many CTAs are in flight together.
+// stream has stored once the CTA has passed a barrier.  A CTA takes some steps of one row: nothing depends on the other
+// CTAs.
 template <typename T>
 struct GradSlice {
     static constexpr int N = Elem<T>::N;
-    Slice<T> in;
+    const T* x;
     T* out;
-    int before, nv, j0;
-    bool same;      // rows of both tensors start at the same place of a vector
+    int V, before, begin, end;      // vectors are those of the output; [begin, end) are this CTA's
+    int full0, full1;               // whole ones of the row
+    bool same;                      // rows of both tensors start at the same place of a vector
 
-    // vectors are those of the output; `chunk` of THREADS * UNROLL of them
-    __device__ __forceinline__ GradSlice(const T* x, T* out_, int V, int chunk) : in(x, V, 0, 1), out(out_) {
+    __device__ __forceinline__ GradSlice(const T* x_, T* out_, int V_, int chunk, int steps) : x(x_), out(out_), V(V_) {
         before = static_cast<int>((reinterpret_cast<uintptr_t>(out_) & 15) / sizeof(T));
-        nv = (before + V + N - 1) / N;
-        j0 = chunk * THREADS * UNROLL;
-        same = before == in.before;
+        same = before == static_cast<int>((reinterpret_cast<uintptr_t>(x_) & 15) / sizeof(T));
+        const int nv = (before + V + N - 1) / N;
+        begin = min(nv, chunk * steps * (THREADS * UNROLL));
+        end = min(nv, begin + steps * (THREADS * UNROLL));
+        full0 = before > 0 ? 1 : 0;
+        full1 = (before + V) / N;
     }
-    __device__ __forceinline__ bool has(long long id) const {
-        if (id < 0 || id >= in.V) return false;
-        const int j = (static_cast<int>(id) + before) / N;
-        return j >= j0 && j < j0 + THREADS * UNROLL;
+    __device__ __forceinline__ bool has(int id) const {
+        const int j = (id + before) / N;
+        return id >= 0 && id < V && j >= begin && j < end;
     }
-    __device__ __forceinline__ bool whole(int j) const { return j * N >= before && j * N + N - before <= in.V; }
-    __device__ __forceinline__ uint4 load(int j) const {
-        if (same && whole(j)) return in.load(j);
-        uint4 r = Slice<T>::nothing();
-        T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int v = j * N + i - before;
-            if (v >= 0 && v < in.V) e[i] = in.row[v];
-        }
-        return r;
+    __device__ __forceinline__ bool smooth(int j) const {       // a step that begins at vector j has whole ones only
+        return j >= full0 && j + THREADS * UNROLL <= min(end, full1);
     }
-    __device__ __forceinline__ void store(int j, const float (&f)[N]) const {
-        if (whole(j)) {
-            *reinterpret_cast<uint4*>(out - before + static_cast<long long>(j) * N) = Elem<T>::pack(f);
-            return;
-        }
+    __device__ __forceinline__ const T* at(const T* p, int j) const { return p - before + static_cast<long long>(j) * N; }
+    __device__ __forceinline__ void load_step(int j0, uint4 (&v)[UNROLL]) const {
+        const int j = j0 + threadIdx.x;
+        if (same && smooth(j0)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int v = j * N + i - before;
-            if (v >= 0 && v < in.V) out[v] = Elem<T>::from(f[i]);
-        }
-    }
-    // out_j = f(x_j)
-    template <typename F>
-    __device__ __forceinline__ void map(F&& f) const {
-        uint4 v[UNROLL];
+            for (int u = 0; u < UNROLL; ++u)
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w) : "l"(at(x, j + u * THREADS)));
+        } else {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int j = j0 + u * THREADS + threadIdx.x;
-            if (j < nv) v[u] = load(j);
-        }
+            for (int u = 0; u < UNROLL; ++u) {
+                const int q = j + u * THREADS;
+                if (q >= end) continue;
+                if (same && q >= full0 && q < full1) {
+                    v[u] = *reinterpret_cast<const uint4*>(at(x, q));
+                    continue;
+                }
+                T* e = reinterpret_cast<T*>(&v[u]);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int j = j0 + u * THREADS + threadIdx.x;
-            if (j < nv) {
-                float x[N];
-                Elem<T>::unpack(v[u], x);
-#pragma unroll
-                for (int e = 0; e < N; ++e) x[e] = f(x[e]);
-                store(j, x);
+                for (int i = 0; i < N; ++i) {
+                    const int k = q * N + i - before;
+                    e[i] = k >= 0 && k < V ? x[k] : Elem<T>::from(0.f);
+                }
             }
         }
     }
-    __device__ __forceinline__ void zero() const {
-        const float z[N] = {};
+    __device__ __forceinline__ void store_step(int j0, const uint4 (&v)[UNROLL]) const {
+        const int j = j0 + threadIdx.x;
+        if (smooth(j0)) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int j = j0 + u * THREADS + threadIdx.x;
-            if (j < nv) store(j, z);
+            for (int u = 0; u < UNROLL; ++u) *reinterpret_cast<uint4*>(const_cast<T*>(at(out, j + u * THREADS))) = v[u];
+        } else {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int q = j + u * THREADS;
+                if (q >= end) continue;
+                if (q >= full0 && q < full1) {
+                    *reinterpret_cast<uint4*>(const_cast<T*>(at(out, q))) = v[u];
+                    continue;
+                }
+                const T* e = reinterpret_cast<const T*>(&v[u]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int k = q * N + i - before;
+                    if (k >= 0 && k < V) out[k] = e[i];
+                }
+            }
         }
+    }
+    // out_j = f(x_j), two at a time; the next step's loads on their way
+    template <typename F>
+    __device__ __forceinline__ void map(F&& f) const {
+        uint4 v[UNROLL], next[UNROLL];
+        if (begin < end) load_step(begin, v);
+        for (int j = begin; j < end; j += THREADS * UNROLL) {
+            if (j + THREADS * UNROLL < end) load_step(j + THREADS * UNROLL, next);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                float e[N];
+                Elem<T>::unpack(v[u], e);
+#pragma unroll
+                for (int i = 0; i < N; i += 2) {
+                    const float2 y = halves(f(pair(e[i], e[i + 1])));
+                    e[i] = y.x;
+                    e[i + 1] = y.y;
+                }
+                v[u] = Elem<T>::pack(e);
+            }
+            store_step(j, v);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) v[u] = next[u];
+        }
+    }
+    __device__ __forceinline__ void zero() const {
+        const uint4 z[UNROLL] = {};
+        for (int j = begin; j < end; j += THREADS * UNROLL) store_step(j, z);
     }
 };
 
@@ -704,7 +1043,7 @@ struct ScoreGradArgs {
     const long long* tokens;
     long long ignore_index;
     float inv_temperature;
-    int k, chunks;
+    int k, chunks, steps;           // CTAs per row, and steps of a CTA
     const float* stats;
     const long long* top_ids;
     const float *d_logprobs, *d_entropy, *d_top;        // any may be null
@@ -712,28 +1051,30 @@ struct ScoreGradArgs {
 
 // dx_j = (1 / temperature) (d_tok (1[tok = j] - p_j) - d_ent p_j (log p_j + H) + sum_i d_top_i (1[id_i = j] - p_j))
 template <typename T>
-__global__ void __launch_bounds__(THREADS) token_logprobs_grad_kernel(const __grid_constant__ ScoreGradArgs p) {
+__global__ void __launch_bounds__(THREADS, 4) token_logprobs_grad_kernel(const __grid_constant__ ScoreGradArgs p) {
     __shared__ float red[32];
     const int tid = threadIdx.x;
-    const long long r = blockIdx.x / p.chunks;
+    const long long r = blockIdx.x / static_cast<unsigned>(p.chunks);
     const int V = p.rows.V;
     T* out = static_cast<T*>(p.grad) + r * V;
-    const GradSlice<T> g(p.rows.row<T>(r), out, V, static_cast<int>(blockIdx.x - r * p.chunks));
+    const GradSlice<T> g(p.rows.row<T>(r), out, V, blockIdx.x % static_cast<unsigned>(p.chunks), p.steps);
     const float4 st = *reinterpret_cast<const float4*>(p.stats + 4 * r);
     const float m = st.x, inv_s = 1.f / st.y, c = p.inv_temperature * LOG2E;
-    long long tok = -1;
+    int tok = -1;
     float d_tok = 0.f;
     if (p.d_logprobs != nullptr) {
-        tok = p.tokens[r];
-        if (tok == p.ignore_index || tok < 0 || tok >= V) tok = -1;
-        else d_tok = p.d_logprobs[r] * p.inv_temperature;
+        const long long i = p.tokens[r];
+        if (i != p.ignore_index && i >= 0 && i < V) {
+            tok = static_cast<int>(i);
+            d_tok = p.d_logprobs[r] * p.inv_temperature;
+        }
     }
     const float d_ent = p.d_entropy != nullptr ? p.d_entropy[r] * p.inv_temperature : 0.f;
-    long long id = -1;
+    int id = -1;
     float d_id = 0.f, d_all = d_tok;
     if (p.d_top != nullptr) {
         if (tid < p.k) {
-            id = p.top_ids[r * p.k + tid];
+            id = static_cast<int>(p.top_ids[r * p.k + tid]);
             d_id = p.d_top[r * p.k + tid] * p.inv_temperature;
         }
         d_all += block_sum(d_id, red);
@@ -741,16 +1082,22 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_grad_kernel(const __gr
     // p_j (a + b log p_j), log p_j = ln2 t_j - log S
     const float a = -(d_all + d_ent * st.z), b = -d_ent;
     const float a2 = inv_s * (a - b * st.w), b2 = inv_s * b * static_cast<float>(LN2);
-    auto value = [&](float x) {
-        const float t = max_nan((x - m) * c, T_MIN);
-        return exp2_approx(t) * fmaf(b2, t, a2);
+    const unsigned long long nm = pair(-m, -m), cc = pair(c, c), aa = pair(a2, a2), bb = pair(b2, b2);
+    auto value = [&](unsigned long long x) {
+        float2 t = halves(mul2(add2(x, nm), cc));
+        t.x = max_nan(t.x, T_MIN);
+        t.y = max_nan(t.y, T_MIN);
+        return mul2(pair(exp2_approx(t.x), exp2_approx(t.y)), fma2(bb, pair(t.x, t.y), aa));
+    };
+    auto value_at = [&](int i) {
+        const float x = Elem<T>::f(g.x[i]);
+        return halves(value(pair(x, x))).x;
     };
     g.map(value);
-    bool met = false;
-    if (p.d_top != nullptr && id >= 0 && g.has(id)) met = id == tok;
+    const bool here = g.has(id), met = here && id == tok;
     const bool taken = __syncthreads_or(met);
-    if (p.d_top != nullptr && id >= 0 && g.has(id)) out[id] = Elem<T>::from(value(Elem<T>::f(g.in.row[id])) + d_id + (met ? d_tok : 0.f));
-    if (tid == 0 && !taken && tok >= 0 && g.has(tok)) out[tok] = Elem<T>::from(value(Elem<T>::f(g.in.row[tok])) + d_tok);
+    if (here) out[id] = Elem<T>::from(value_at(id) + d_id + (met ? d_tok : 0.f));
+    if (tid == 0 && !taken && g.has(tok)) out[tok] = Elem<T>::from(value_at(tok) + d_tok);
 }
 
 // ------------------------------------------------------------------ distillation from a teacher's best tokens
@@ -767,7 +1114,7 @@ struct DistillArgs {
     const long long* labels;        // or null
     long long ignore_index;
     double inv_temperature;
-    int k, splits, forward_kl, tail;
+    int k, splits, stages, forward_kl, tail;
     float *kl, *nll;
     int* entries;                   // [rows][k]: the ids that count, -1 elsewhere
     float* stats;                   // [rows][8]
@@ -783,23 +1130,29 @@ struct DistillPart {        // of a CTA, relative to its largest logit m
     double px;              // METHOD 1: sum of listed exponentials times (x / temperature - teacher's log)
 };
 
-template <typename T, bool TWO>
-__global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
+template <typename T, AtOne ONE>
+__global__ void __launch_bounds__(THREADS, 3) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
     constexpr int N = Elem<T>::N;
-    extern __shared__ __align__(16) uint32_t listed[];      // a byte per vector of this CTA
+    extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then a byte per vector of this CTA
+    uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + ring_bytes(p.stages));
     __shared__ float red[4 * WARPS];
     __shared__ int id_of[MAX_K];
     __shared__ DistillPart part;
-    __shared__ double part_of[WARPS][4];
+    __shared__ double part_of[MAX_K / 32][4];
+    __shared__ float list_max[2][MAX_K / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long r = blockIdx.x / p.splits;
-    const int rank = blockIdx.x - static_cast<int>(r * p.splits);
+    const long long r = blockIdx.x / static_cast<unsigned>(p.splits);
+    const int rank = blockIdx.x % static_cast<unsigned>(p.splits);
     const int V = p.rows.V;
     const T* row = p.rows.row<T>(r);
     const Slice<T> sl(row, V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
 
+    Ring<T> ring(sl, vocab_smem, p.stages);
     // the list: entries that count are in the vocabulary, have a finite or NaN value, and come first of their token
+    static_assert(UNROLL == 4, "a word of the map has a lane's vectors of a step");
+    const int words = (sl.full1 - sl.full0 + WARP_STEP - 1) / WARP_STEP * 32;       // and one each for the parts at the ends
+    for (int i = tid; i < words + 2; i += THREADS) listed[i] = 0;
     int id = -1;
     float lq = -INFINITY;
     if (tid < p.k) {
@@ -811,7 +1164,8 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
     const long long label = p.labels != nullptr ? p.labels[r] : p.ignore_index;
     const bool labelled = label != p.ignore_index;
     const bool any = __syncthreads_or(id >= 0);
-    if (!any && !labelled) {            // nothing is asked of this row: it is not read
+    if (!any && !labelled) {            // nothing is asked of this row: it is not read, but for what the ring has under way
+        ring.drain();
         if (rank == 0) {
             if (tid < p.k) p.entries[r * p.k + tid] = -1;
             if (tid == 0) {
@@ -822,155 +1176,181 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
         }
         return;                         // (all CTAs of the cluster alike)
     }
-    const int words = (sl.end - sl.begin + 3) / 4;
-    for (int i = tid; i < words; i += THREADS) listed[i] = 0;
-    __syncthreads();
     const bool mine = id >= 0 && sl.has(id);
     bool again = false;
     if (mine) {
-        const int j = (id + sl.before) / N - sl.begin, bit = (j & 3) * 8 + (id + sl.before) % N;
-        again = atomicOr(&listed[j >> 2], 1u << bit) >> bit & 1u;
+        const int j = (id + sl.before) / N, q = j - sl.full0;
+        const int word = sl.whole(j) ? q / WARP_STEP * 32 + q % 32 : words + (j == 0 ? 0 : 1);
+        const int bit = (sl.whole(j) ? q % WARP_STEP / 32 * 8 : 0) + (id + sl.before) % N;
+        again = atomicOr(&listed[word], 1u << bit) >> bit & 1u;
     }
     bool counts = mine;
     if (__syncthreads_or(again) && mine)
         for (int i = 0; i < tid; ++i) counts &= id_of[i] != id;
     if (tid < p.k && (mine || (rank == 0 && id < 0))) p.entries[r * p.k + tid] = counts ? id : -1;
+    const float x = counts ? Elem<T>::f(row[id]) : -INFINITY;
+    const float x_label = rank == 0 && tid == 0 && labelled && label >= 0 && label < V ? Elem<T>::f(row[label]) : 0.f;
 
-    Running<false, TWO> run;
-    const uint8_t* flag = reinterpret_cast<const uint8_t*>(listed);
-    const int steps = sl.steps();
-    auto hide = [&](uint4& v, int j) {
-        const uint32_t b = flag[j - sl.begin];
-        if (b != 0) {
-            T* e = reinterpret_cast<T*>(&v);
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (b >> i & 1u) e[i] = Elem<T>::from(-INFINITY);
-        }
-    };
-    for (int step = 0; step < steps; ++step) {
-        uint4 v[UNROLL];
-        const int j0 = sl.full0 + step * THREADS * UNROLL + tid;
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) v[u] = j0 + u * THREADS < sl.full1 ? sl.load(j0 + u * THREADS) : Slice<T>::nothing();
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (j0 + u * THREADS < sl.full1) hide(v[u], j0 + u * THREADS);
-        run.template add<T>(v, max_of<T>(v), c, LOG2E);
-    }
+    Running<false, ONE> run;
+    ring.stream(
+        [&](int step, uint32_t address) {
+            uint32_t bits = listed[(step * WARPS + warp) * 32 + lane];
+            if (bits != 0) {        // a lane's own vectors, which it reads next
+                for (; bits != 0; bits &= bits - 1) {
+                    const int b = __ffs(bits) - 1;
+                    const uint32_t at = address + b / 8 * 512 + b % 8 * static_cast<int>(sizeof(T));
+                    if constexpr (sizeof(T) == 2)
+                        asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(static_cast<uint16_t>(Elem<T>::NEG_INF & 0xffffu)) : "memory");
+                    else
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(Elem<T>::NEG_INF) : "memory");
+                }
+                fence_proxy_async_smem();
+            }
+        },
+        [&](int, uint4 (&v)[UNROLL], bool whole) {
+            run.template add<T>(v, whole, [&] { return max_of<T>(v); }, c, LOG2E);
+        });
     if ((tid == 0 && sl.head) || (tid == 1 && sl.tail)) {
-        const int j = tid == 0 ? 0 : sl.nv - 1;
-        uint4 v[1] = {sl.load_part(j)};
-        hide(v[0], j);
-        run.template add<T>(v, max_of<T>(v), c, LOG2E);
+        uint4 v[1] = {sl.load_part(tid == 0 ? 0 : sl.nv - 1)};
+        T* e = reinterpret_cast<T*>(&v[0]);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (listed[words + tid] >> i & 1u) e[i] = Elem<T>::from(-INFINITY);
+        run.template add<T>(v, false, [&] { return max_of<T>(v); }, c, LOG2E);
     }
     Sums sum = join_block(run, c, LOG2E, red);
 
     // the listed tokens, in 64 bits.  Weights without a tail are relative to the largest value of the list.
-    const float x = counts ? Elem<T>::f(row[id]) : -INFINITY;
     float m = max_nan(x, -INFINITY), ref = id >= 0 ? lq : -INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        ref = max_nan(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-    }
-    __syncthreads();
-    if (lane == 0) {
-        red[warp] = m;
-        red[WARPS + warp] = ref;
-    }
-    __syncthreads();
-    for (int i = 0; i < MAX_K / 32; ++i) {
-        m = max_nan(m, red[i]);
-        ref = max_nan(ref, red[WARPS + i]);
-    }
-    m = max_nan(m, sum.m);
-    if (p.tail || ref == -INFINITY) ref = 0.f;
-    double e[4] = {0, 0, 0, 0};         // listed exponentials, at temperature one, weights, products
-    if (counts) {
-        const double d = static_cast<double>(x) - m, y = static_cast<double>(x) * p.inv_temperature;
-        e[0] = x == -INFINITY ? 0.0 : exp(d * p.inv_temperature);
-        e[1] = TWO ? (x == -INFINITY ? 0.0 : exp(d)) : 0.0;
-        e[2] = exp(static_cast<double>(lq) - ref);
-        if (p.forward_kl) e[3] = e[0] == 0.0 ? 0.0 : e[0] * (y - lq);
-        else e[3] = e[2] == 0.0 ? 0.0 : e[2] * (static_cast<double>(lq) - ref - y);
-    }
     if (warp < MAX_K / 32) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int o = 16; o > 0; o >>= 1) {
+            m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+            ref = max_nan(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+        }
+        if (lane == 0) {
+            list_max[0][warp] = m;
+            list_max[1][warp] = ref;
+        }
+    }
+    __syncthreads();
+    if (warp < MAX_K / 32) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) e[q] += __shfl_xor_sync(0xffffffffu, e[q], o);
+        for (int i = 0; i < MAX_K / 32; ++i) {
+            m = max_nan(m, list_max[0][i]);
+            ref = max_nan(ref, list_max[1][i]);
+        }
+        m = max_nan(m, sum.m);
+        if (p.tail || ref == -INFINITY) ref = 0.f;
+        double e[4] = {0, 0, 0, 0};     // listed exponentials, at temperature one, weights, products
+        if (counts) {
+            const double d = static_cast<double>(x) - m, y = static_cast<double>(x) * p.inv_temperature;
+            e[0] = x == -INFINITY ? 0.0 : exp(d * p.inv_temperature);
+            if (ONE) e[1] = x == -INFINITY ? 0.0 : exp(d);
+            e[2] = exp(static_cast<double>(lq) - ref);
+            if (p.forward_kl) e[3] = e[0] == 0.0 ? 0.0 : e[0] * (y - lq);
+            else e[3] = e[2] == 0.0 ? 0.0 : e[2] * (static_cast<double>(lq) - ref - y);
+        }
+        if (p.k > 32 * warp) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (ONE || q != 1)
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) e[q] += __shfl_xor_sync(0xffffffffu, e[q], o);
+        }
         if (lane == 0)
             for (int q = 0; q < 4; ++q) part_of[warp][q] = e[q];
     }
     const int n = __syncthreads_count(counts);
+    if (warp > 0 && p.splits == 1) return;
     if (tid == 0) {
+        double e[4];
         for (int q = 0; q < 4; ++q) {
             e[q] = 0;
             for (int i = 0; i < MAX_K / 32; ++i) e[q] += part_of[i][q];
         }
-        const double d = sum.m == m ? 0.0 : fmax(static_cast<double>(sum.m) - m, -1e30);
-        const double f = exp(d * p.inv_temperature);
-        part = DistillPart{m, n, sum.s * f, e[0], TWO ? sum.s1 * exp(d) + e[1] : 0.0, e[2], p.forward_kl ? 0.0 : e[3],
-                           p.forward_kl ? e[3] : 0.0};
+        double rest = sum.s, rest1 = sum.s1;
+        if (sum.m != m) {
+            const double d = fmax(static_cast<double>(sum.m) - m, -1e30);
+            rest *= exp(d * p.inv_temperature);
+            if (ONE) rest1 *= exp(d);
+        }
+        part = DistillPart{m, n, rest, e[0], ONE ? rest1 + e[1] : 0.0, e[2], p.forward_kl ? 0.0 : e[3], p.forward_kl ? e[3] : 0.0};
     }
+    __syncwarp();
     if (p.splits > 1) cluster_sync();
-    if (rank == 0 && tid == 0) {
+    if (rank == 0 && warp == 0) {
         DistillPart all = part;
-        if (p.splits > 1) {
-            for (int q = 1; q < p.splits; ++q) all.m = max_nan(all.m, ld_peer(&part.m, q));
-            all.n = 0;
-            all.rest = all.top = all.all1 = all.q = all.qx = all.px = 0;
-            for (int q = 0; q < p.splits; ++q) {
-                const float mq = ld_peer(&part.m, q);
-                const double d = mq == all.m ? 0.0 : fmax(static_cast<double>(mq) - all.m, -1e30);
-                const double f = exp(d * p.inv_temperature);
-                all.n += ld_peer(&part.n, q);
-                all.rest += ld_peer(&part.rest, q) * f;
-                all.top += ld_peer(&part.top, q) * f;
-                all.px += ld_peer(&part.px, q) * f;
-                if (TWO) all.all1 += ld_peer(&part.all1, q) * exp(d);
-                all.q += ld_peer(&part.q, q);
-                all.qx += ld_peer(&part.qx, q);
+        if (p.splits > 1) {             // a lane for each part
+            const bool there = lane < p.splits;
+            const DistillPart* q = &part;
+            all.m = there ? ld_peer(&q->m, lane) : -INFINITY;
+            all.n = there ? ld_peer(&q->n, lane) : 0;
+            all.rest = there ? ld_peer(&q->rest, lane) : 0;
+            all.top = there ? ld_peer(&q->top, lane) : 0;
+            all.all1 = there && ONE ? ld_peer(&q->all1, lane) : 0;
+            all.q = there ? ld_peer(&q->q, lane) : 0;
+            all.qx = there ? ld_peer(&q->qx, lane) : 0;
+            all.px = there ? ld_peer(&q->px, lane) : 0;
+            float largest = all.m;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            if (there && all.m != largest) {
+                const double d = fmax(static_cast<double>(all.m) - largest, -1e30), f = exp(d * p.inv_temperature);
+                all.rest *= f;
+                all.top *= f;
+                all.px *= f;
+                if (ONE) all.all1 *= exp(d);
+            }
+            all.m = largest;
+            double* v[6] = {&all.rest, &all.top, &all.all1, &all.q, &all.qx, &all.px};
+#pragma unroll
+            for (int o = MAX_SPLITS / 2; o > 0; o >>= 1) {
+                all.n += __shfl_xor_sync(0xffffffffu, all.n, o);
+#pragma unroll
+                for (int i = 0; i < 6; ++i) *v[i] += __shfl_xor_sync(0xffffffffu, *v[i], o);
             }
         }
-        const double S = all.rest + all.top, log_s = log(S), lse = all.m * p.inv_temperature + log_s;
-        const double S1 = TWO ? all.all1 : S;
-        double kl = 0, factor = 0, fourth = 0, norm = 0;
-        if (all.n > 0) {
-            const double p_r = all.rest / S, log_p_r = log(p_r);
-            double q_r = 0;
-            if (p.tail) {
-                q_r = 1 - all.q;
-                if (q_r < NO_TAIL) q_r = 0;
-            }
-            if (!p.forward_kl) {
-                if (p.tail) {
-                    kl = all.qx + all.q * lse;
-                    if (q_r > 0) kl += q_r * (log(q_r) - log_p_r);
-                    fourth = all.q + q_r;
+        // the logarithms, a lane for each, then one thread
+        const double S = all.rest + all.top, S1 = ONE ? all.all1 : S;
+        double q_r = p.tail ? 1 - all.q : 0.0;
+        if (q_r < NO_TAIL) q_r = 0;
+        const double logs = log(lane == 0 ? S : lane == 1 ? all.rest : lane == 2 ? fmax(q_r, NO_TAIL) : lane == 3 ? all.q : S1);
+        const double log_s = __shfl_sync(0xffffffffu, logs, 0), log_p_r = __shfl_sync(0xffffffffu, logs, 1) - log_s;
+        const double log_q_r = __shfl_sync(0xffffffffu, logs, 2), log_q = __shfl_sync(0xffffffffu, logs, 3);
+        const double log_s1 = __shfl_sync(0xffffffffu, logs, 4);
+        if (lane == 0) {
+            const double lse = all.m * p.inv_temperature + log_s;
+            double kl = 0, factor = 0, fourth = 0, norm = 0;
+            if (all.n > 0) {
+                const double p_r = all.rest / S;
+                if (!p.forward_kl) {
+                    if (p.tail) {
+                        kl = all.qx + all.q * lse;
+                        if (q_r > 0) kl += q_r * (log_q_r - log_p_r);
+                        fourth = all.q + q_r;
+                    } else {
+                        norm = ref + log_q;
+                        kl = all.qx / all.q - log_q + lse;
+                        fourth = 1;
+                    }
+                    factor = fourth - (p_r > 0 ? q_r / p_r : 0.0);
                 } else {
-                    norm = ref + log(all.q);
-                    kl = all.qx / all.q - log(all.q) + lse;
-                    fourth = 1;
+                    const double ratio = p_r > 0 ? log_p_r - log_q_r : 0.0;
+                    kl = (all.px - all.top * lse) / S + p_r * ratio;
+                    fourth = kl;
+                    factor = ratio - kl;
                 }
-                factor = fourth - (p_r > 0 ? q_r / p_r : 0.0);
-            } else {
-                const double ratio = p_r > 0 ? log_p_r - log(fmax(q_r, NO_TAIL)) : 0.0;
-                kl = (all.px - all.top * lse) / S + p_r * ratio;
-                fourth = kl;
-                factor = ratio - kl;
             }
+            p.kl[r] = static_cast<float>(kl);
+            if (p.nll != nullptr)
+                p.nll[r] = !labelled              ? 0.f
+                           : label >= 0 && label < V ? static_cast<float>(log_s1 - (static_cast<double>(x_label) - all.m))
+                                                     : __int_as_float(0x7fffffff);
+            float4* st = reinterpret_cast<float4*>(p.stats + 8 * r);
+            st[0] = make_float4(all.m, static_cast<float>(1 / S), static_cast<float>(factor), static_cast<float>(fourth));
+            st[1] = make_float4(static_cast<float>(norm), static_cast<float>(1 / S1), static_cast<float>(log_s), 1.f);
         }
-        p.kl[r] = static_cast<float>(kl);
-        if (p.nll != nullptr)
-            p.nll[r] = !labelled ? 0.f
-                       : label >= 0 && label < V
-                           ? static_cast<float>(log(S1) - (static_cast<double>(Elem<T>::f(row[label])) - all.m))
-                           : __int_as_float(0x7fffffff);
-        float4* st = reinterpret_cast<float4*>(p.stats + 8 * r);
-        st[0] = make_float4(all.m, static_cast<float>(1 / S), static_cast<float>(factor), static_cast<float>(fourth));
-        st[1] = make_float4(static_cast<float>(norm), static_cast<float>(1 / S1), static_cast<float>(log_s), 1.f);
     }
     if (p.splits > 1) cluster_sync();
 }
@@ -983,20 +1363,20 @@ struct DistillGradArgs {
     const long long* labels;
     long long ignore_index;
     float inv_temperature;
-    int k, chunks, forward_kl;
+    int k, chunks, steps, forward_kl;
     const float* stats;
     const float *d_kl, *d_nll;      // either may be null
 };
 
 // Tokens that are not listed: p_j times the row's factor.  Listed ones: p_i (sum q + q_r) - q_i (METHOD 0),
 // p_i (log p_i - log q_i - KL) (METHOD 1).  Both over the temperature, and the cross entropy's p_j - 1[label = j] on top.
-template <typename T, bool TWO>
-__global__ void __launch_bounds__(THREADS) topk_distillation_grad_kernel(const __grid_constant__ DistillGradArgs p) {
+template <typename T, AtOne ONE>
+__global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(const __grid_constant__ DistillGradArgs p) {
     const int tid = threadIdx.x;
-    const long long r = blockIdx.x / p.chunks;
+    const long long r = blockIdx.x / static_cast<unsigned>(p.chunks);
     const int V = p.rows.V;
     T* out = static_cast<T*>(p.grad) + r * V;
-    const GradSlice<T> g(p.rows.row<T>(r), out, V, static_cast<int>(blockIdx.x - r * p.chunks));
+    const GradSlice<T> g(p.rows.row<T>(r), out, V, blockIdx.x % static_cast<unsigned>(p.chunks), p.steps);
     const float4 s0 = reinterpret_cast<const float4*>(p.stats + 8 * r)[0], s1 = reinterpret_cast<const float4*>(p.stats + 8 * r)[1];
     if (s1.w == 0.f) {              // no loss: not read, gradient zero
         g.zero();
@@ -1004,44 +1384,54 @@ __global__ void __launch_bounds__(THREADS) topk_distillation_grad_kernel(const _
     }
     const float m = s0.x, inv_s = s0.y, c = p.inv_temperature * LOG2E;
     const float d_kl = p.d_kl != nullptr ? p.d_kl[r] * p.inv_temperature : 0.f;
-    long long label = -1;
+    int label = -1;
     float d_nll = 0.f;
     if (p.d_nll != nullptr) {
-        label = p.labels[r];
-        if (label == p.ignore_index || label < 0 || label >= V) label = -1;
-        else d_nll = p.d_nll[r];
+        const long long i = p.labels[r];
+        if (i != p.ignore_index && i >= 0 && i < V) {
+            label = static_cast<int>(i);
+            d_nll = p.d_nll[r];
+        }
     }
-    const float a = d_kl * inv_s * s0.z + (TWO ? 0.f : d_nll * inv_s), a1 = d_nll * s1.y;
-    auto t_of = [&](float x) { return max_nan((x - m) * c, T_MIN); };
-    auto e1_of = [&](float x) { return exp2_approx(max_nan((x - m) * LOG2E, T_MIN)); };
-    auto value = [&](float x) {
-        const float v = exp2_approx(t_of(x)) * a;
-        return TWO ? fmaf(e1_of(x), a1, v) : v;
+    const float a = d_kl * inv_s * s0.z + (ONE ? 0.f : d_nll * inv_s), a1 = d_nll * s1.y;
+    const unsigned long long nm = pair(-m, -m), cc = pair(c, c), cc1 = pair(LOG2E, LOG2E), aa = pair(a, a), aa1 = pair(a1, a1);
+    auto t_of = [&](float x) { return (x - m) * c; };
+    auto value = [&](unsigned long long x) {
+        const unsigned long long d = add2(x, nm);
+        const float2 t = halves(mul2(d, cc));
+        const unsigned long long e = pair(exp2_approx(t.x), exp2_approx(t.y)), v = mul2(e, aa);
+        if (ONE == NONE) return v;
+        if (ONE == SQUARE) return fma2(mul2(e, e), aa1, v);
+        const float2 t1 = halves(mul2(d, cc1));
+        return fma2(pair(exp2_approx(t1.x), exp2_approx(t1.y)), aa1, v);
     };
     g.map(value);
     int id = -1;
     if (tid < p.k) id = p.entries[r * p.k + tid];
-    const bool here = id >= 0 && g.has(id), met = here && id == label;
+    const bool here = g.has(id), met = here && id == label;
     const bool taken = __syncthreads_or(met);
     if (here) {
-        const float x = Elem<T>::f(g.in.row[id]), t = t_of(x), e = exp2_approx(t) * inv_s;
+        const float x = Elem<T>::f(g.x[id]), t = t_of(x), e = exp2_approx(t) * inv_s;
         const float lq = p.teacher[r * p.k + tid] - s1.x;
         float v;
         if (p.forward_kl) v = e == 0.f ? 0.f : e * (t * static_cast<float>(LN2) - s1.z - lq - s0.w);
         else v = e * s0.w - __expf(lq);
-        v = v * d_kl + d_nll * (TWO ? e1_of(x) * s1.y : e) - (met ? d_nll : 0.f);
+        v = v * d_kl + d_nll * (ONE ? exp2_approx((x - m) * LOG2E) * s1.y : e) - (met ? d_nll : 0.f);
         out[id] = Elem<T>::from(v);
     }
-    if (tid == 0 && !taken && label >= 0 && g.has(label)) out[label] = Elem<T>::from(value(Elem<T>::f(g.in.row[label])) - d_nll);
+    if (tid == 0 && !taken && g.has(label)) {
+        const float x = Elem<T>::f(g.x[label]);
+        out[label] = Elem<T>::from(halves(value(pair(x, x))).x - d_nll);
+    }
 }
 
 // ------------------------------------------------------------------ launches
-// CTAs per row: one when there are rows for every SM, else as many as it takes to give each SM about two, while a CTA
-// keeps a step of work.
+// CTAs per row: as many as fit on the GPU at once (three per SM) for all rows, while each keeps a step of work.  250 x 32000
+// fp32 logits, distillation forward: 13 us with one, 18 with two; 333 x 32000 bf16, scores: 9.1 with one, 12.2 with two.
 inline int splits_for(long long rows, int V, int elem) {
     const int step = THREADS * 16 / elem;
     int n = 1;
-    while (n < MAX_SPLITS && rows * n < 296 && V > step * n) n *= 2;
+    while (n < MAX_SPLITS && rows * n * 2 <= 148 * 3 && V > step * n) n *= 2;
     return n;
 }
 
@@ -1062,9 +1452,30 @@ inline cudaError_t launch(Kern kern, const Args& a, long long ctas, int splits, 
 }
 
 inline int elem_size(int dtype) { return dtype == LME_F32 ? 4 : 2; }
-inline int chunks_for(int V, int elem) {     // of a gradient row, whose first vector may be a part
-    const int n = 16 / elem;
-    return (V + 2 * n - 2 + n * THREADS * UNROLL - 1) / (n * THREADS * UNROLL);
+// Steps of a gradient's CTA: four, so that what it has to know of its row costs little, fewer where that would leave SMs
+// idle.
+struct GradGrid {
+    int chunks, steps;
+};
+inline GradGrid grad_grid(long long rows, int V, int elem) {
+    const int n = 16 / elem, step = THREADS * UNROLL;
+    const int vectors = static_cast<int>((V + 2ll * n - 2) / n), all = (vectors + step - 1) / step;   // the first may be a part
+    int steps = 4;
+    while (steps > 1 && rows * ((all + steps - 1) / steps) < 148 * 8) steps /= 2;
+    return {(all + steps - 1) / steps, steps};
+}
+// Dynamic shared memory of the streaming kernels; the attribute is set to the most that any call asks for.
+constexpr int RING_STAGES = 2;
+constexpr int MAX_SMEM = ring_bytes(RING_STAGES) + MAX_MAP;
+template <typename T>
+inline cudaError_t launch_score(const ScoreArgs& a, long long ctas, void* stream) {
+    const bool top = a.k > 0;
+    const int smem = max(ring_bytes(a.stages), top ? static_cast<int>(sizeof(Selection)) : 0);
+    if (!(top ? opt_in<token_logprobs_kernel<T, true>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM)
+              : opt_in<token_logprobs_kernel<T, false>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM)))
+        return cudaErrorInvalidValue;
+    return top ? launch(token_logprobs_kernel<T, true>, a, ctas, a.splits, smem, stream)
+               : launch(token_logprobs_kernel<T, false>, a, ctas, a.splits, smem, stream);
 }
 constexpr long long MAX_GRID = 0x7fffffff;
 constexpr int MAX_V = 1 << 30;
@@ -1080,21 +1491,15 @@ extern "C" int lme_token_logprobs_fwd(const void* x, int dtype, long long rows, 
     if (dtype < LME_BF16 || dtype > LME_F32 || rows < 0 || inner < 1 || V < 1 || k < 0 || k > MAX_K || k > V || !(temperature > 0))
         return LME_ERR_SHAPE;
     if (rows == 0) return LME_OK;
+    if (V > MAX_V || rows > MAX_GRID) return LME_ERR_TOO_LARGE;
     const int splits = splits_for(rows, V, elem_size(dtype));
-    if (V > MAX_V || rows * splits > MAX_GRID) return LME_ERR_TOO_LARGE;
-    const ScoreArgs a{{x, inner, ld_inner, ld_outer, V}, tokens, ignore_index, 1.0 / temperature, k, splits, logprobs, entropy,
+    if (rows * splits > MAX_GRID) return LME_ERR_TOO_LARGE;
+    const ScoreArgs a{{x, inner, ld_inner, ld_outer, V}, tokens, ignore_index, 1.0 / temperature, k, splits, RING_STAGES, logprobs, entropy,
                       top_logprobs, top_ids, stats};
     const long long ctas = rows * splits;
-    cudaError_t e;
-    if (dtype == LME_BF16)
-        e = k > 0 ? launch(token_logprobs_kernel<__nv_bfloat16, true>, a, ctas, splits, 0, stream)
-                  : launch(token_logprobs_kernel<__nv_bfloat16, false>, a, ctas, splits, 0, stream);
-    else if (dtype == LME_F16)
-        e = k > 0 ? launch(token_logprobs_kernel<__half, true>, a, ctas, splits, 0, stream)
-                  : launch(token_logprobs_kernel<__half, false>, a, ctas, splits, 0, stream);
-    else
-        e = k > 0 ? launch(token_logprobs_kernel<float, true>, a, ctas, splits, 0, stream)
-                  : launch(token_logprobs_kernel<float, false>, a, ctas, splits, 0, stream);
+    const cudaError_t e = dtype == LME_BF16  ? launch_score<__nv_bfloat16>(a, ctas, stream)
+                          : dtype == LME_F16 ? launch_score<__half>(a, ctas, stream)
+                                             : launch_score<float>(a, ctas, stream);
     return e == cudaSuccess ? LME_LAUNCH_OK() : LME_ERR_LAUNCH;
 }
 
@@ -1108,11 +1513,12 @@ extern "C" int lme_token_logprobs_bwd(const void* x, int dtype, long long rows, 
         (d_logprobs != nullptr && tokens == nullptr))
         return LME_ERR_SHAPE;
     if (rows == 0) return LME_OK;
-    const int chunks = chunks_for(V, elem_size(dtype));
-    if (V > MAX_V || rows * chunks > MAX_GRID) return LME_ERR_TOO_LARGE;
+    if (V > MAX_V) return LME_ERR_TOO_LARGE;
+    const GradGrid grid = grad_grid(rows, V, elem_size(dtype));
+    if (rows * grid.chunks > MAX_GRID) return LME_ERR_TOO_LARGE;
     const ScoreGradArgs a{{x, inner, ld_inner, ld_outer, V}, grad, tokens, ignore_index, static_cast<float>(1.0 / temperature), k,
-                          chunks, stats, top_ids, d_logprobs, d_entropy, d_top};
-    const long long ctas = rows * chunks;
+                          grid.chunks, grid.steps, stats, top_ids, d_logprobs, d_entropy, d_top};
+    const long long ctas = rows * grid.chunks;
     const cudaError_t e = dtype == LME_BF16  ? launch(token_logprobs_grad_kernel<__nv_bfloat16>, a, ctas, 1, 0, stream)
                           : dtype == LME_F16 ? launch(token_logprobs_grad_kernel<__half>, a, ctas, 1, 0, stream)
                                              : launch(token_logprobs_grad_kernel<float>, a, ctas, 1, 0, stream);
@@ -1121,20 +1527,23 @@ extern "C" int lme_token_logprobs_bwd(const void* x, int dtype, long long rows, 
 
 namespace lme {
 namespace vr {
-template <typename T>
-inline cudaError_t launch_distill(const DistillArgs& a, bool two, long long ctas, int splits, int smem, void* stream) {
-    if (smem > 48 * 1024) {
-        const bool ok = two ? opt_in<topk_distillation_kernel<T, true>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_MAP)
-                            : opt_in<topk_distillation_kernel<T, false>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_MAP);
-        if (!ok) return cudaErrorInvalidValue;
-    }
-    return two ? launch(topk_distillation_kernel<T, true>, a, ctas, splits, smem, stream)
-               : launch(topk_distillation_kernel<T, false>, a, ctas, splits, smem, stream);
+inline AtOne at_one(bool labels, double temperature) { return !labels || temperature == 1.0 ? NONE : temperature == 2.0 ? SQUARE : OWN; }
+template <typename T, AtOne ONE>
+inline cudaError_t launch_distill_one(const DistillArgs& a, long long ctas, int smem, void* stream) {
+    if (!opt_in<topk_distillation_kernel<T, ONE>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM)) return cudaErrorInvalidValue;
+    return launch(topk_distillation_kernel<T, ONE>, a, ctas, a.splits, smem, stream);
 }
 template <typename T>
-inline cudaError_t launch_distill_grad(const DistillGradArgs& a, bool two, long long ctas, void* stream) {
-    return two ? launch(topk_distillation_grad_kernel<T, true>, a, ctas, 1, 0, stream)
-               : launch(topk_distillation_grad_kernel<T, false>, a, ctas, 1, 0, stream);
+inline cudaError_t launch_distill(const DistillArgs& a, AtOne one, long long ctas, int smem, void* stream) {
+    return one == NONE  ? launch_distill_one<T, NONE>(a, ctas, smem, stream)
+           : one == OWN ? launch_distill_one<T, OWN>(a, ctas, smem, stream)
+                        : launch_distill_one<T, SQUARE>(a, ctas, smem, stream);
+}
+template <typename T>
+inline cudaError_t launch_distill_grad(const DistillGradArgs& a, AtOne one, long long ctas, void* stream) {
+    return one == NONE  ? launch(topk_distillation_grad_kernel<T, NONE>, a, ctas, 1, 0, stream)
+           : one == OWN ? launch(topk_distillation_grad_kernel<T, OWN>, a, ctas, 1, 0, stream)
+                        : launch(topk_distillation_grad_kernel<T, SQUARE>, a, ctas, 1, 0, stream);
 }
 }  // namespace vr
 }  // namespace lme
@@ -1148,20 +1557,20 @@ extern "C" int lme_topk_distillation_fwd(const void* x, int dtype, long long row
         (forward_kl && !tail) || (labels != nullptr) != (nll != nullptr))
         return LME_ERR_SHAPE;
     if (rows == 0) return LME_OK;
+    if (V > MAX_V || rows > MAX_GRID) return LME_ERR_TOO_LARGE;
     const int n = 16 / elem_size(dtype);
     int splits = splits_for(rows, V, elem_size(dtype));
-    auto map_bytes = [&](int s) { return (((V + 2 * n - 2) / n + s - 1) / s + 3 + 16) / 16 * 16; };
-    if (V > MAX_V) return LME_ERR_TOO_LARGE;
+    auto map_bytes = [&](int s) { return ((((V + 2 * n - 2) / n + s - 1) / s + WARP_STEP - 1) / WARP_STEP * 32 + 4) * 4; };
     while (splits < MAX_SPLITS && map_bytes(splits) > MAX_MAP) splits *= 2;
     if (map_bytes(splits) > MAX_MAP || rows * splits > MAX_GRID) return LME_ERR_TOO_LARGE;
     const DistillArgs a{{x, inner, ld_inner, ld_outer, V}, top_ids, top_logprobs, labels, ignore_index, 1.0 / temperature, k,
-                        splits, forward_kl, tail, kl, nll, entries, stats};
-    const bool two = labels != nullptr && temperature != 1.0;
+                        splits, RING_STAGES, forward_kl, tail, kl, nll, entries, stats};
+    const AtOne one = at_one(labels != nullptr, temperature);
     const long long ctas = rows * splits;
-    const int smem = map_bytes(splits);
-    const cudaError_t e = dtype == LME_BF16  ? launch_distill<__nv_bfloat16>(a, two, ctas, splits, smem, stream)
-                          : dtype == LME_F16 ? launch_distill<__half>(a, two, ctas, splits, smem, stream)
-                                             : launch_distill<float>(a, two, ctas, splits, smem, stream);
+    const int smem = ring_bytes(a.stages) + map_bytes(splits);
+    const cudaError_t e = dtype == LME_BF16  ? launch_distill<__nv_bfloat16>(a, one, ctas, smem, stream)
+                          : dtype == LME_F16 ? launch_distill<__half>(a, one, ctas, smem, stream)
+                                             : launch_distill<float>(a, one, ctas, smem, stream);
     return e == cudaSuccess ? LME_LAUNCH_OK() : LME_ERR_LAUNCH;
 }
 
@@ -1174,14 +1583,15 @@ extern "C" int lme_topk_distillation_bwd(const void* x, int dtype, long long row
         (d_nll != nullptr && labels == nullptr))
         return LME_ERR_SHAPE;
     if (rows == 0) return LME_OK;
-    const int chunks = chunks_for(V, elem_size(dtype));
-    if (V > MAX_V || rows * chunks > MAX_GRID) return LME_ERR_TOO_LARGE;
+    if (V > MAX_V) return LME_ERR_TOO_LARGE;
+    const GradGrid grid = grad_grid(rows, V, elem_size(dtype));
+    if (rows * grid.chunks > MAX_GRID) return LME_ERR_TOO_LARGE;
     const DistillGradArgs a{{x, inner, ld_inner, ld_outer, V}, grad, entries, top_logprobs, labels, ignore_index,
-                            static_cast<float>(1.0 / temperature), k, chunks, forward_kl, stats, d_kl, d_nll};
-    const bool two = d_nll != nullptr && temperature != 1.0;
-    const long long ctas = rows * chunks;
-    const cudaError_t e = dtype == LME_BF16  ? launch_distill_grad<__nv_bfloat16>(a, two, ctas, stream)
-                          : dtype == LME_F16 ? launch_distill_grad<__half>(a, two, ctas, stream)
-                                             : launch_distill_grad<float>(a, two, ctas, stream);
+                            static_cast<float>(1.0 / temperature), k, grid.chunks, grid.steps, forward_kl, stats, d_kl, d_nll};
+    const AtOne one = at_one(d_nll != nullptr, temperature);
+    const long long ctas = rows * grid.chunks;
+    const cudaError_t e = dtype == LME_BF16  ? launch_distill_grad<__nv_bfloat16>(a, one, ctas, stream)
+                          : dtype == LME_F16 ? launch_distill_grad<__half>(a, one, ctas, stream)
+                                             : launch_distill_grad<float>(a, one, ctas, stream);
     return e == cudaSuccess ? LME_LAUNCH_OK() : LME_ERR_LAUNCH;
 }

@@ -168,15 +168,25 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_is_tracing = torch._C._is_tracing
+_len_torch_dispatch_stack = torch._C._len_torch_dispatch_stack
+_peek_interpreter_stack = torch._C._functorch.peek_interpreter_stack
+
+
 def eager(*tensors: torch.Tensor) -> bool:
     """Whether kernels may take these tensors by address: plain tensors of the current device, outside tracing,
     functorch transforms, forward-mode AD and dispatch modes, all of which need operations that they can see."""
-    if (torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack()
-            or torch.autograd.forward_ad._current_level >= 0
-            or torch._C._functorch.peek_interpreter_stack() is not None):
+    if (torch.compiler.is_compiling() or _is_tracing() or _len_torch_dispatch_stack()
+            or torch.autograd.forward_ad._current_level >= 0 or _peek_interpreter_stack() is not None):
         return False
-    return all((type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and t.is_cuda for t in tensors) and all(
-        t.get_device() == torch._C._cuda_getDevice() for t in tensors)
+    for t in tensors:
+        if (type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda:
+            return False
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != device:
+            return False
+    return True
 
 
 def strides(t: torch.Tensor) -> tuple[int, ...]:

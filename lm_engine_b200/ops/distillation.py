@@ -14,7 +14,7 @@ import torch.nn.functional as F
 
 from ..enums import KLDivergenceMethod
 from . import _lib
-from .logprobs import KERNEL_TYPES, MAX_TOP_K, check_logits, check_tokens, kernel_usable, logit_rows
+from .logprobs import KERNEL_TYPES, MAX_TOP_K, as_int64, check_logits, check_tokens, integers, kernel_usable, logit_rows
 
 #: The teacher's mass outside of its listed tokens is one minus their sum, which the rounding of fp32 log probabilities moves by
 #: about this much: a smaller rest counts as none, and as this much where its logarithm is asked for.
@@ -81,26 +81,31 @@ class _TopkDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index):
         x, inner, ld_inner, ld_outer = logit_rows(logits)
-        shape, dev = logits.shape[:-1], logits.device
-        K = top_ids.size(-1)
-        kl = torch.empty(shape, dtype=torch.float32, device=dev)
-        nll = torch.empty(shape, dtype=torch.float32, device=dev) if labels is not None else None
-        entries = torch.empty((*shape, K), dtype=torch.int32, device=dev)
-        stats = torch.empty((*shape, 8), dtype=torch.float32, device=dev)
-        _lib.check(_lib.cuda_lib().lme_topk_distillation_fwd(
-            x.data_ptr(), KERNEL_TYPES[x.dtype], kl.numel(), inner, ld_inner, ld_outer, x.size(-1), top_ids.data_ptr(),
+        K, V = top_ids.size(-1), x.size(-1)
+        rows = x.numel() // V
+        if labels is None:
+            kl, nll = torch.empty(tuple(x.shape[:-1]), dtype=torch.float32, device=x.device), None
+        else:                               # (empty_like costs half of what a shape and a device do)
+            kl = torch.empty_like(labels, dtype=torch.float32)
+            nll = torch.empty_like(kl)
+        ctx.entries = torch.empty_like(top_ids, dtype=torch.int32)
+        ctx.stats = torch.empty(8 * rows, dtype=torch.float32, device=x.device)
+        rc = _lib.cuda_lib().lme_topk_distillation_fwd(
+            x.data_ptr(), KERNEL_TYPES[x.dtype], rows, inner, ld_inner, ld_outer, V, top_ids.data_ptr(),
             top_logprobs.data_ptr(), K, _lib.ptr(labels), ignore_index, temperature,
-            int(method == KLDivergenceMethod.forward), int(tail), kl.data_ptr(), _lib.ptr(nll), entries.data_ptr(),
-            stats.data_ptr(), _lib.stream_ptr()), "lme_topk_distillation_fwd")
+            method is KLDivergenceMethod.forward, tail, kl.data_ptr(), _lib.ptr(nll), ctx.entries.data_ptr(),
+            ctx.stats.data_ptr(), _lib.stream_ptr())
+        if rc:
+            _lib.check(rc, "lme_topk_distillation_fwd")
         _lib.count_launch()
-        ctx.save_for_backward(logits, top_ids, top_logprobs, labels, entries, stats)
+        ctx.save_for_backward(logits, top_ids, top_logprobs, labels)
         ctx.meta = (method, tail, temperature, ignore_index)
         ctx.set_materialize_grads(False)
         return kl, nll
 
     @staticmethod
     def backward(ctx, d_kl, d_nll):
-        logits, top_ids, top_logprobs, labels, entries, stats = ctx.saved_tensors
+        logits, top_ids, top_logprobs, labels = ctx.saved_tensors
         method, tail, temperature, ignore_index = ctx.meta
         nothing = (None,) * 7
         if d_kl is None and d_nll is None:
@@ -110,16 +115,18 @@ class _TopkDistillation(torch.autograd.Function):
             outs = topk_distillation_reference(x, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index)
             outs, grads = zip(*((o, g) for o, g in zip(outs, (d_kl, d_nll)) if g is not None))
             return *torch.autograd.grad(outs, [x], grads, create_graph=True), *nothing
-        d_kl, d_nll = (None if g is None else g.float().contiguous() for g in (d_kl, d_nll))
         x, inner, ld_inner, ld_outer = logit_rows(logits)
-        top_logprobs, labels, entries, stats = (None if t is None else _lib.aligned(t)
-                                                for t in (top_logprobs, labels, entries, stats))
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _lib.check(_lib.cuda_lib().lme_topk_distillation_bwd(
-            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // x.size(-1), inner, ld_inner, ld_outer, x.size(-1),
-            entries.data_ptr(), top_logprobs.data_ptr(), entries.size(-1), _lib.ptr(labels), ignore_index, temperature,
-            int(method == KLDivergenceMethod.forward), stats.data_ptr(), _lib.ptr(d_kl), _lib.ptr(d_nll),
-            grad.data_ptr(), _lib.stream_ptr()), "lme_topk_distillation_bwd")
+        V = x.size(-1)
+        top_logprobs, labels, d_kl, d_nll = (None if t is None else t.contiguous()
+                                             for t in (top_logprobs, labels, d_kl, d_nll))
+        grad = torch.empty_like(x, memory_format=torch.contiguous_format)
+        rc = _lib.cuda_lib().lme_topk_distillation_bwd(
+            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // V, inner, ld_inner, ld_outer, V, ctx.entries.data_ptr(),
+            top_logprobs.data_ptr(), top_ids.size(-1), _lib.ptr(labels), ignore_index, temperature,
+            method is KLDivergenceMethod.forward, ctx.stats.data_ptr(), _lib.ptr(d_kl), _lib.ptr(d_nll),
+            grad.data_ptr(), _lib.stream_ptr())
+        if rc:
+            _lib.check(rc, "lme_topk_distillation_bwd")
         _lib.count_launch()
         return grad, *nothing
 
@@ -149,7 +156,9 @@ def topk_distillation(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs:
     K = top_ids.size(-1) if top_ids.dim() else 0
     if not 1 <= K <= MAX_TOP_K:
         raise ValueError(f"a teacher's list has 1..{MAX_TOP_K} tokens, got top_ids of {tuple(top_ids.shape)}")
-    check_tokens("top_ids", top_ids[..., 0], logits)
+    if top_ids.shape[:-1] != logits.shape[:-1] or not integers(top_ids):
+        raise ValueError(f"top_ids have to be integers of shape {tuple(logits.shape[:-1])} and the list, got "
+                         f"{top_ids.dtype} of {tuple(top_ids.shape)}")
     if top_logprobs.shape != top_ids.shape or not top_logprobs.is_floating_point():
         raise ValueError(f"top_logprobs need a floating type and shape {tuple(top_ids.shape)}, got {top_logprobs.dtype} of "
                          f"{tuple(top_logprobs.shape)}")
@@ -158,7 +167,7 @@ def topk_distillation(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs:
     if not kernel_usable(logits, temperature, top_ids, top_logprobs, labels):
         return topk_distillation_reference(logits, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index)
     if labels is not None:
-        labels = labels.to(torch.int64).contiguous()
+        labels = as_int64(labels)
     return TopkDistillation(*_TopkDistillation.apply(
-        logits, top_ids.to(torch.int64).contiguous(), top_logprobs.detach().float().contiguous(), labels, method,
-        bool(tail), float(temperature), int(ignore_index)))
+        logits, as_int64(top_ids), top_logprobs.detach().float().contiguous(), labels, method, bool(tail),
+        float(temperature), int(ignore_index)))

@@ -69,8 +69,9 @@ def logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
 
 def kernel_usable(logits: torch.Tensor, temperature, *others: torch.Tensor | None) -> bool:
     """A temperature that is a tensor may want a gradient: it is left to the PyTorch operations."""
-    return (logits.dtype in KERNEL_TYPES and not isinstance(temperature, torch.Tensor)
-            and logits.size(-1) <= 1 << 30 and _lib.eager(logits, *(t for t in others if t is not None)))
+    if logits.dtype not in KERNEL_TYPES or isinstance(temperature, torch.Tensor) or logits.size(-1) > 1 << 30:
+        return False
+    return _lib.eager(logits, *[t for t in others if t is not None])
 
 
 def check_logits(logits: torch.Tensor, temperature) -> None:
@@ -80,24 +81,43 @@ def check_logits(logits: torch.Tensor, temperature) -> None:
         raise ValueError(f"temperature has to be positive, got {temperature}")
 
 
+def integers(t: torch.Tensor) -> bool:
+    return t.dtype == torch.int64 or not (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool)
+
+
+def as_int64(t: torch.Tensor) -> torch.Tensor:
+    return t.contiguous() if t.dtype == torch.int64 else t.to(torch.int64).contiguous()
+
+
 def check_tokens(name: str, tokens: torch.Tensor, logits: torch.Tensor) -> None:
-    if tokens.shape != logits.shape[:-1] or tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+    if tokens.shape != logits.shape[:-1] or not integers(tokens):
         raise ValueError(f"{name} have to be integers of shape {tuple(logits.shape[:-1])}, got {tokens.dtype} of "
                          f"{tuple(tokens.shape)}")
 
 
 def _forward(logits, tokens, top_k, temperature, ignore_index, with_stats):
     x, inner, ld_inner, ld_outer = logit_rows(logits)
-    shape, dev = logits.shape[:-1], logits.device
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
-    logprobs = torch.empty(shape, dtype=torch.float32, device=dev) if tokens is not None else None
-    top = torch.empty((*shape, top_k), dtype=torch.float32, device=dev) if top_k else None
-    ids = torch.empty((*shape, top_k), dtype=torch.int64, device=dev) if top_k else None
-    stats = torch.empty((*shape, 4), dtype=torch.float32, device=dev) if with_stats else None
-    _lib.check(_lib.cuda_lib().lme_token_logprobs_fwd(
-        x.data_ptr(), KERNEL_TYPES[x.dtype], entropy.numel(), inner, ld_inner, ld_outer, x.size(-1), _lib.ptr(tokens),
-        ignore_index, temperature, top_k, _lib.ptr(logprobs), entropy.data_ptr(), _lib.ptr(top), _lib.ptr(ids),
-        _lib.ptr(stats), _lib.stream_ptr()), "lme_token_logprobs_fwd")
+    shape = x.shape
+    V = shape[-1]
+    rows = x.numel() // V
+    logprobs = top = ids = stats = None
+    if tokens is not None:              # (empty_like costs half of what a shape and a device do)
+        logprobs = torch.empty_like(tokens, dtype=torch.float32)
+        entropy = torch.empty_like(logprobs)
+    else:
+        entropy = torch.empty(tuple(shape[:-1]), dtype=torch.float32, device=x.device)
+    if top_k:
+        top = torch.empty((*shape[:-1], top_k), dtype=torch.float32, device=x.device)
+        ids = torch.empty_like(top, dtype=torch.int64)
+    if with_stats:
+        stats = torch.empty(4 * rows, dtype=torch.float32, device=x.device)
+    rc = _lib.cuda_lib().lme_token_logprobs_fwd(
+        x.data_ptr(), KERNEL_TYPES[x.dtype], rows, inner, ld_inner, ld_outer, V,
+        None if tokens is None else tokens.data_ptr(), ignore_index, temperature, top_k,
+        None if tokens is None else logprobs.data_ptr(), entropy.data_ptr(), top.data_ptr() if top_k else None,
+        ids.data_ptr() if top_k else None, stats.data_ptr() if with_stats else None, _lib.stream_ptr())
+    if rc:
+        _lib.check(rc, "lme_token_logprobs_fwd")
     _lib.count_launch()
     return logprobs, entropy, top, ids, stats
 
@@ -105,34 +125,35 @@ def _forward(logits, tokens, top_k, temperature, ignore_index, with_stats):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
-        logprobs, entropy, top, ids, stats = _forward(logits, tokens, top_k, temperature, ignore_index, True)
-        ctx.save_for_backward(logits, tokens, ids, stats)
+        logprobs, entropy, top, ids, ctx.stats = _forward(logits, tokens, top_k, temperature, ignore_index, True)
+        ctx.save_for_backward(logits, tokens, ids)
         ctx.meta = (top_k, temperature, ignore_index)
         ctx.set_materialize_grads(False)
-        if ids is not None:
+        if top_k:
             ctx.mark_non_differentiable(ids)
         return logprobs, entropy, top, ids
 
     @staticmethod
     def backward(ctx, d_logprobs, d_entropy, d_top, _):
-        logits, tokens, ids, stats = ctx.saved_tensors
+        logits, tokens, ids = ctx.saved_tensors
         top_k, temperature, ignore_index = ctx.meta
-        grads = (d_logprobs, d_entropy, d_top)
-        if all(g is None for g in grads):
+        if d_logprobs is None and d_entropy is None and d_top is None:
             return None, None, None, None, None
         if torch.is_grad_enabled():         # a graph of the gradients is asked for
             x = logits.view_as(logits)
             outs = token_logprobs_reference(x, tokens, top_k, temperature, ignore_index)[:3]
-            outs, grads = zip(*((o, g) for o, g in zip(outs, grads) if g is not None))
+            outs, grads = zip(*((o, g) for o, g in zip(outs, (d_logprobs, d_entropy, d_top)) if g is not None))
             return *torch.autograd.grad(outs, [x], grads, create_graph=True), None, None, None, None
-        d_logprobs, d_entropy, d_top = (None if g is None else g.float().contiguous() for g in grads)
         x, inner, ld_inner, ld_outer = logit_rows(logits)
-        tokens, ids, stats = (None if t is None else _lib.aligned(t) for t in (tokens, ids, stats))
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _lib.check(_lib.cuda_lib().lme_token_logprobs_bwd(
-            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // x.size(-1), inner, ld_inner, ld_outer, x.size(-1),
-            _lib.ptr(tokens), ignore_index, temperature, top_k, stats.data_ptr(), _lib.ptr(ids), _lib.ptr(d_logprobs),
-            _lib.ptr(d_entropy), _lib.ptr(d_top), grad.data_ptr(), _lib.stream_ptr()), "lme_token_logprobs_bwd")
+        V = x.size(-1)
+        small = [None if t is None else t.contiguous() for t in (tokens, ids, d_logprobs, d_entropy, d_top)]
+        grad = torch.empty_like(x, memory_format=torch.contiguous_format)
+        rc = _lib.cuda_lib().lme_token_logprobs_bwd(
+            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // V, inner, ld_inner, ld_outer, V, _lib.ptr(small[0]),
+            ignore_index, temperature, top_k, ctx.stats.data_ptr(), *[_lib.ptr(t) for t in small[1:]],
+            grad.data_ptr(), _lib.stream_ptr())
+        if rc:
+            _lib.check(rc, "lme_token_logprobs_bwd")
         _lib.count_launch()
         return grad, None, None, None, None
 
@@ -157,7 +178,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     if not kernel_usable(logits, temperature, tokens):
         return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)
     if tokens is not None:
-        tokens = tokens.to(torch.int64).contiguous()
+        tokens = as_int64(tokens)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, int(top_k), float(temperature), int(ignore_index)))
     return TokenLogprobs(*_forward(logits, tokens, int(top_k), float(temperature), int(ignore_index), False)[:4])
