@@ -272,10 +272,18 @@ class TeacherArgs(BaseArgs):
     dtype: str = "fp32"
     kl_divergence_method: KLDivergenceMethod | None = None
     kl_divergence_weight: float = 1
+    # extension: distil from the teacher's that many most likely tokens per position (with the rest of the vocabulary as
+    # one more outcome, or renormalised over the list) instead of from its whole distribution
+    kl_divergence_top_k: int | None = None
+    kl_divergence_tail: bool = True
 
     def model_post_init(self, _ctx: Any) -> None:
         self.dtype = normalize_dtype_string(self.dtype)
         _require(kl_divergence_method=self.kl_divergence_method)
+        if self.kl_divergence_top_k is not None:
+            assert 1 <= self.kl_divergence_top_k <= 128, "kl_divergence_top_k has to be in 1..128"
+            assert self.kl_divergence_tail or self.kl_divergence_method == KLDivergenceMethod.backward, (
+                "kl_divergence_method forward needs kl_divergence_tail")
 
 
 class TrainingArgs(BaseArgs):

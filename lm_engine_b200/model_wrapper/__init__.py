@@ -47,7 +47,8 @@ def get_model_container(args: TrainingArgs | DistillationArgs, efficient_initial
         t = args.teacher_args
         kwargs.update(teacher_model_name=t.model_name, teacher_pretrained_config=t.pretrained_config,
                       teacher_model_dtype=t.dtype, kl_divergence_method=t.kl_divergence_method,
-                      kl_divergence_weight=t.kl_divergence_weight,
+                      kl_divergence_weight=t.kl_divergence_weight, kl_divergence_top_k=t.kl_divergence_top_k,
+                      kl_divergence_tail=t.kl_divergence_tail,
                       micro_batch_size=args.training_parameters.micro_batch_size,
                       sequence_length=args.datasets[0].class_args.get("sequence_length"))
     cls = _wrapper_class(method)

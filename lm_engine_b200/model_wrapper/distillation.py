@@ -2,7 +2,10 @@
 sees the same tokens (lm_engine/model_wrapper/distillation.py:24-212).
 
 ``kl_divergence_method``: ``forward`` = sum student * ln(student / teacher); ``backward`` = sum teacher *
-ln(teacher / student); both averaged over tokens ("batchmean").  The student is sharded by the engine like any other
+ln(teacher / student); both averaged over tokens ("batchmean").  With ``kl_divergence_top_k`` the teacher is reduced to its
+most likely tokens per position as soon as its logits are there, and the loss, with the labels' cross entropy and the
+gradient, is one pass over the student's logits each way (``ops.topk_distillation``) in place of four fp32 tensors of their
+size; ``kl_divergence_tail`` keeps the rest of the vocabulary as one more outcome.  The student is sharded by the engine like any other
 model; the teacher is a replicated, gradient-free copy in ``teacher_model_dtype`` placed on the device when the
 student is wrapped (B200 keeps an 8B teacher in 16 GB of its 180 GB).  Tensor / pipeline parallel distillation is not
 supported, as in the reference.
@@ -16,9 +19,10 @@ import os
 import torch
 import torch.nn.functional as F
 
+from .. import ops
 from ..enums import KLDivergenceMethod
 from ..logging_utils import log_rank_0
-from ..loss import get_autoregressive_language_modeling_loss
+from ..loss import IGNORE_INDEX, get_autoregressive_language_modeling_loss
 from ..models import CommonConfig, build_model, config_from_dict
 from ..parallel.manager import ProcessGroupManager
 from ..utils import string_to_torch_dtype
@@ -29,13 +33,16 @@ class ModelWrapperForDistillation(ModelWrapperForPretraining):
     def __init__(self, *args, teacher_model_name: str | None = None, teacher_pretrained_config: dict | None = None,
                  teacher_model_dtype: torch.dtype | str = torch.bfloat16,
                  kl_divergence_method: KLDivergenceMethod = KLDivergenceMethod.forward,
-                 kl_divergence_weight: float = 1, **kwargs) -> None:
+                 kl_divergence_weight: float = 1, kl_divergence_top_k: int | None = None,
+                 kl_divergence_tail: bool = True, **kwargs) -> None:
         self.teacher_model_name = teacher_model_name
         self.teacher_pretrained_config = teacher_pretrained_config
         self.teacher_model_dtype = (string_to_torch_dtype(teacher_model_dtype)
                                     if isinstance(teacher_model_dtype, str) else teacher_model_dtype)
         self.kl_divergence_method = KLDivergenceMethod(kl_divergence_method)
         self.kl_divergence_weight = kl_divergence_weight
+        self.kl_divergence_top_k = kl_divergence_top_k
+        self.kl_divergence_tail = kl_divergence_tail
         super().__init__(*args, **kwargs)
         if ProcessGroupManager.is_tensor_parallel_enabled() or self.num_pipeline_stages > 1:
             raise NotImplementedError("distillation supports data parallel sharding only")
@@ -77,6 +84,14 @@ class ModelWrapperForDistillation(ModelWrapperForPretraining):
             batch = {"text": batch}
         inputs, labels = self._prepare_model_inputs(batch)
         student_logits = self.model(**inputs).logits
+        if self.kl_divergence_top_k is not None:
+            with torch.no_grad():
+                best = ops.token_logprobs(self.teacher_model(**inputs).logits, top_k=self.kl_divergence_top_k)
+            out = ops.topk_distillation(student_logits, best.top_ids, best.top_logprobs,
+                                        labels.reshape(student_logits.shape[:-1]), self.kl_divergence_method,
+                                        self.kl_divergence_tail, ignore_index=IGNORE_INDEX)
+            lm_loss, kl = out.nll.sum() * lm_loss_multiplier, out.kl_divergence.mean()
+            return {"loss": lm_loss + self.kl_divergence_weight * kl, "lm_loss": lm_loss, "kl_divergence": kl}
         lm_loss = get_autoregressive_language_modeling_loss(
             lm_logits=student_logits, labels=labels, cu_seqlens=None,
             use_padding_free_transformer=self.use_padding_free_transformer, reduction="sum",

@@ -143,7 +143,7 @@ def test_rows_without_loss_are_not_looked_at():
     ids, lq = torch.tensor([[0], [-1]]), torch.tensor([[-1.0], [-1.0]])
     out = topk_distillation(x, ids, lq, torch.tensor([1, -100]))
     (g,) = torch.autograd.grad(out.kl_divergence.sum() + out.nll.sum(), x)
-    assert float(out.kl_divergence[1]) == float(out.nll[1]) == 0 and torch.equal(g[1], torch.zeros(5, dtype=F64))
+    assert float(out.kl_divergence[1].detach()) == float(out.nll[1].detach()) == 0 and torch.equal(g[1], torch.zeros(5, dtype=F64))
 
 
 def test_places_of_rows():
@@ -201,3 +201,57 @@ def test_entry_points_refuse_on_the_host():
     assert lib.lme_token_logprobs_fwd(None, 0, 1 << 31, 1, 8, 8, 8, None, -100, 1.0, 0, None, None, None, None, None,
                                       None) == -6
     assert lib.lme_token_logprobs_fwd(None, 0, 0, 1, 8, 8, 8, None, -100, 1.0, 0, None, None, None, None, None, None) == 0
+
+
+def _wrapper(top_k, method, tail=True):
+    from lm_engine_b200.model_wrapper.distillation import ModelWrapperForDistillation
+    from lm_engine_b200.models import dense_config
+    from lm_engine_b200.parallel.manager import ProcessGroupManager
+
+    ProcessGroupManager.destroy_process_groups()
+    ProcessGroupManager(zero_stage=0)
+    torch.manual_seed(2)
+
+    def cfg(hidden):
+        return dense_config(vocab_size=96, hidden_size=hidden, num_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                            intermediate_size=64, max_position_embeddings=16).to_dict()
+
+    return ModelWrapperForDistillation(
+        pretrained_config=cfg(32), micro_batch_size=2, sequence_length=16, teacher_pretrained_config=cfg(48),
+        teacher_model_dtype="fp32", kl_divergence_method=method, kl_divergence_weight=0.5, kl_divergence_top_k=top_k,
+        kl_divergence_tail=tail)
+
+
+@pytest.mark.parametrize("method", ["forward", "backward"])
+def test_distillation_training_from_best_tokens(method):
+    """A list of the whole vocabulary is the full divergence; a shorter one is a lower bound of it (data processing)."""
+    tokens = torch.randint(0, 96, (2, 17), generator=torch.Generator().manual_seed(0))
+    results = {}
+    for top_k in (None, 96, 8):
+        w = _wrapper(top_k, method)
+        out = w(tokens, lm_loss_multiplier=1 / 32)
+        out["loss"].backward()
+        grads = [p.grad for p in w.parameters() if p.grad is not None]
+        assert all(p.grad is None for p in w.teacher_model.parameters()) and grads
+        results[top_k] = (out, grads)
+    full, full_grads = results[None]
+    listed, listed_grads = results[96]
+    for name in full:
+        torch.testing.assert_close(listed[name], full[name], rtol=1e-5, atol=1e-6)
+    for a, b in zip(listed_grads, full_grads):
+        torch.testing.assert_close(a, b, rtol=1e-3, atol=1e-6)
+    short = results[8][0]
+    assert 0 < float(short["kl_divergence"].detach()) < float(full["kl_divergence"].detach())
+    torch.testing.assert_close(short["lm_loss"], full["lm_loss"], rtol=1e-5, atol=1e-6)
+
+
+def test_teacher_arguments():
+    from lm_engine_b200.arguments import TeacherArgs
+
+    assert TeacherArgs(model_name="t", kl_divergence_method="forward").kl_divergence_top_k is None
+    assert TeacherArgs(model_name="t", kl_divergence_method="backward", kl_divergence_top_k=64,
+                       kl_divergence_tail=False).kl_divergence_top_k == 64
+    for bad in (dict(kl_divergence_top_k=0), dict(kl_divergence_top_k=129),
+                dict(kl_divergence_top_k=8, kl_divergence_tail=False)):
+        with pytest.raises(Exception):
+            TeacherArgs(model_name="t", kl_divergence_method="forward", **bad)
