@@ -70,11 +70,12 @@ def _score(x, tok, k, temperature, seed=0, grads=True):
     assert got.dtype == x.dtype and got.shape == x.shape
     logp = torch.log_softmax(x64.detach() / temperature, -1)
     p = logp.exp()
-    size = p * sum((d.abs().sum(-1) if d.dim() > p.dim() - 1 else d.abs())[..., None] for _, _, d in pairs)
-    size = size * (2 + logp.clamp(min=-300).abs() + math.log2(V + 1))      # terms that add up to a gradient
-    eps = torch.finfo(x.dtype).eps / 2
-    tiny = 2.0 ** -25 if x.dtype == HF else 2.0 ** -126
-    _check(got, ref, ref.abs().nan_to_num(0) * (eps + 2.0 ** -22) + size.nan_to_num(0) / temperature * (4 * e) + tiny, "gradient")
+    size = sum((d.abs().sum(-1) if d.dim() > p.dim() - 1 else d.abs())[..., None] for _, _, d in pairs)
+    size = (size * (2 + logp.clamp(min=-300).abs() + math.log2(V + 1)) / temperature).nan_to_num(0)     # terms that add up to
+    eps = torch.finfo(x.dtype).eps / 2                                                                # a gradient, over p
+    # an exponential below 2^-126 counts as none: off by that times the same factors (the sum that divides it is one at least)
+    tiny = size * 2.0 ** -126 + (2.0 ** -25 if x.dtype == HF else 2.0 ** -126)
+    _check(got, ref, ref.abs().nan_to_num(0) * (eps + 2.0 ** -22) + (p * size).nan_to_num(0) * (4 * e) + tiny, "gradient")
     return out
 
 
@@ -230,7 +231,10 @@ def _distill(x, ids, lq, labels, method, tail, temperature, seed=0, slack=1.0):
     if labels is not None:
         terms = terms + torch.softmax(x64.detach(), -1) * d[1].abs()[..., None]
     eps = torch.finfo(x.dtype).eps / 2
-    tiny = 2.0 ** -25 if x.dtype == HF else 2.0 ** -126
+    # an exponential below 2^-126 counts as none: off by that times what terms has beside p
+    flushed = (1 + over) if method == "backward" else 4 + 300 + kl.abs()[..., None] + lq.double().abs().clamp(max=1e4).amax(-1, keepdim=True)
+    tiny = 2.0 ** -126 * (flushed * d[0].abs()[..., None] / temperature + 1).nan_to_num(0, 0, 0)
+    tiny = tiny + (2.0 ** -25 if x.dtype == HF else 2.0 ** -126)
     _check(got, ref, ref.abs().nan_to_num(0) * (eps + 2.0 ** -22) + terms.nan_to_num(0) * (4 * e * slack) + tiny, "gradient")
     return out, got
 
@@ -464,3 +468,132 @@ def test_a_long_batch_passes_32_bits():
     want = 9 - math.log(math.exp(9) + V - 1)
     assert float((out.logprobs - want).abs().max()) < _sum_error(V) + 2.0 ** -22
     assert torch.equal(out.top_ids[:, 0], tok) and torch.equal(out.top_ids[1:, 1], torch.zeros_like(tok[1:]))
+
+
+@pytest.mark.parametrize("rows", [1, 500])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_rows_whose_logits_leave_the_range_of_their_first_ones(rows, dtype):
+    """A thread's sums run over (values hundreds above its first ones), meet minus infinity or the type's lowest late in the
+    row, or begin with them."""
+    V = 30011
+    x = _rows(1, rows, V, dtype, 11)
+    tok = torch.full((1, rows), V - 3, device="cuda")
+    ids, lq = _lists(x, 12, 2)
+    low = torch.finfo(dtype).min
+    cases = []
+    for first in (-400.0, -90.0):
+        y = x.clone()
+        y[..., : 2 * V // 3] += first
+        cases.append(y)
+    y = x.clone()
+    y[..., V // 2:] += 300.0
+    y[..., ::7] = -math.inf
+    cases.append(y)
+    for value in (-math.inf, low):
+        y = x.clone()
+        y[..., 17000:] = value
+        cases.append(y)
+        y = x.clone()
+        y[..., :17000] = value
+        cases.append(y)
+    y = torch.full_like(x, low)                     # all forbidden by the lowest value: as likely as each other
+    cases.append(y)
+    y = y.clone()
+    y[..., 5::2] = -math.inf
+    cases.append(y)
+    if dtype != HF:
+        cases.append(x + 4000)
+    for y in cases:
+        y = y.clone()
+        y[..., V - 3] = y[..., :].amax(-1)
+        _score(y, tok, 20, 1.0)
+        _score(y, tok, 0, 0.7)
+    for y in cases[:6]:
+        y = y.clone()
+        keep = y.gather(-1, ids)
+        y.scatter_(-1, ids, torch.where(keep > -80, keep, 0.0).to(dtype))       # (listed ones stay likely: finite losses)
+        _distill(y, ids, lq, ids[..., 0], "backward", False, 2.0)
+        _distill(y, ids, lq, ids[..., 0], "backward", False, 1.3)
+        _distill(y, ids, lq, None, "forward", True, 1.0)
+
+
+@pytest.mark.parametrize("rows,V", [(700, 9001), (2000, 12001)])
+def test_many_calls_give_the_same_bits(rows, V):
+    """Stages of the ring are requested again while their last values are in use nearby."""
+    from lm_engine_b200.ops import token_logprobs, topk_distillation
+
+    x = _rows(1, rows, V, F32, 3)
+    ids, lq = _lists(x, 16, 4)
+    first = None
+    for _ in range(300):
+        a = [*token_logprobs(x, ids[..., 0], top_k=1), *topk_distillation(x, ids, lq, ids[..., 1])]
+        first = first or a
+        assert all(torch.equal(u, v) for u, v in zip(first, a))
+
+
+def test_kernels_are_what_runs():
+    from lm_engine_b200.ops import _lib, token_logprobs, topk_distillation
+
+    for dtype in (BF, HF, F32):
+        x = _rows(1, 3, 515, dtype, 1, "odd start").requires_grad_(True)
+        ids, lq = _lists(x.detach(), 4, 1)
+        before = _lib.launch_count
+        token_logprobs(x, ids[..., 0], top_k=2).entropy.sum().backward()
+        topk_distillation(x, ids, lq, ids[..., 0]).nll.sum().backward()
+        assert _lib.launch_count == before + 4
+    assert _lib.read_status()[0] == 0
+
+
+def test_teacher_to_student():
+    """The two together as a distillation step uses them: the teacher's best tokens, the loss, the student's gradient."""
+    from lm_engine_b200.ops import token_logprobs, token_logprobs_reference, topk_distillation, topk_distillation_reference
+
+    teacher, student = _rows(2, 100, 32000, BF, 1), _rows(2, 100, 32000, BF, 2).requires_grad_(True)
+    labels = torch.randint(32000, (2, 100), device="cuda")
+    labels[0, :40] = -100
+    best = token_logprobs(teacher, top_k=64)
+    out = topk_distillation(student, best.top_ids, best.top_logprobs, labels)
+    (got,) = torch.autograd.grad(out.kl_divergence.mean() + out.nll.sum() / 160, student)
+    x64 = student.detach().double().requires_grad_(True)
+    t64 = token_logprobs_reference(teacher.double(), top_k=64)
+    want = topk_distillation_reference(x64, t64.top_ids, t64.top_logprobs, labels)
+    (ref,) = torch.autograd.grad(want.kl_divergence.mean() + want.nll.sum() / 160, x64)
+    e = _sum_error(32000)
+    assert torch.equal(best.top_ids, t64.top_ids)
+    # the list's error reaches the divergence through its weights, times its logarithms (at most 2 log2 V)
+    assert float((out.kl_divergence - want.kl_divergence).abs().max()) < 30 * e
+    assert float((out.nll - want.nll).abs().max()) < e + 20 * 2.0 ** -23
+    assert float((got.double() - ref).norm() / ref.norm()) < 2.0 ** -8      # half a step of bf16, and 30 e
+
+
+@pytest.mark.parametrize("method", ["forward", "backward"])
+def test_distillation_wrapper(method):
+    from lm_engine_b200.model_wrapper.distillation import ModelWrapperForDistillation
+    from lm_engine_b200.models import dense_config
+    from lm_engine_b200.ops import _lib, token_logprobs_reference, topk_distillation_reference
+    from lm_engine_b200.parallel.manager import ProcessGroupManager
+
+    ProcessGroupManager.destroy_process_groups()
+    ProcessGroupManager(zero_stage=0)
+    torch.manual_seed(3)
+
+    def cfg(hidden):
+        return dense_config(vocab_size=512, hidden_size=hidden, num_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                            intermediate_size=256, head_dim=64, max_position_embeddings=64).to_dict()
+
+    w = ModelWrapperForDistillation(
+        pretrained_config=cfg(128), micro_batch_size=2, sequence_length=64, teacher_pretrained_config=cfg(256),
+        teacher_model_dtype="bf16", kl_divergence_method=method, kl_divergence_weight=0.5, kl_divergence_top_k=32,
+        dtype="bf16").cuda()
+    w.place_teacher(torch.device("cuda"))
+    tokens = torch.randint(0, 512, (2, 65), device="cuda")
+    out = w(tokens, lm_loss_multiplier=1 / 128)
+    out["loss"].backward()
+    s, t = (m(input_ids=tokens[:, :-1]).logits.double() for m in (w.model, w.teacher_model))
+    best = token_logprobs_reference(t, top_k=32)
+    want = topk_distillation_reference(s, best.top_ids, best.top_logprobs, tokens[:, 1:], method)
+    e = _sum_error(512) * 60
+    assert abs(float(out["kl_divergence"]) - float(want.kl_divergence.mean())) < e
+    assert abs(float(out["lm_loss"]) - float(want.nll.mean())) < e
+    assert all(p.grad is not None and torch.isfinite(p.grad.float()).all() for p in w.model.parameters())
+    assert all(p.grad is None for p in w.teacher_model.parameters()) and _lib.read_status()[0] == 0
