@@ -186,7 +186,7 @@ struct Slice {
     __device__ __forceinline__ Slice(const T* row_, int V_, int rank, int splits) : row(row_), V(V_) {
         before = static_cast<int>((reinterpret_cast<uintptr_t>(row_) & 15) / sizeof(T));
         nv = (before + V + N - 1) / N;
-        const int per = (nv + splits - 1) / splits;
+        const int per = splits == 1 ? nv : (nv + splits - 1) / splits;
         begin = min(nv, rank * per);
         end = min(nv, begin + per);
         const bool ragged = (before + V) % N != 0;
@@ -548,8 +548,8 @@ struct Selection {
 __device__ __noinline__ int order_candidates(Selection& sel, int n, int k) {
     const int tid = threadIdx.x;
     if (n <= THREADS) {             // the place of a candidate is the number of those ahead of it: some lanes count for each
-        const int lanes = n <= THREADS / 8 ? 8 : n <= THREADS / 4 ? 4 : n <= THREADS / 2 ? 2 : 1;
-        const int at = tid / lanes, part = tid % lanes;
+        const int shift = n <= THREADS / 8 ? 3 : n <= THREADS / 4 ? 2 : n <= THREADS / 2 ? 1 : 0, lanes = 1 << shift;
+        const int at = tid >> shift, part = tid & (lanes - 1);
         const unsigned long long mine = at < n ? sel.cand[at] : 0;
         int ahead = 0;
 #pragma unroll 4
@@ -722,7 +722,7 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
 // hardly more (1.2 k for k = 64 where values come in no order), so only the segments that do are read again.  Few
 // instructions matter more than few reads: the other CTAs of the SM stream meanwhile, and a warp gets every eighth slot.
 template <typename T>
-__device__ __noinline__ int select_best(Selection& sel, const float* group, const Slice<T>& sl, int k, float largest, int segment_steps) {
+__device__ __noinline__ int select_best(Selection& sel, const float* group, const Slice<T>& sl, int k, float largest, int segment_shift) {
     constexpr int N = Elem<T>::N, AHEAD = 4;
     const int tid = threadIdx.x;
     find_reach(sel, largest, k);
@@ -735,7 +735,8 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
             sel.chosen[at++] = static_cast<unsigned short>((__ffs(mask) - 1) * THREADS + tid);
     }
     __syncthreads();
-    const int per = max(segment_steps, 1) * UNROLL, items = sel.groups * per;
+    const int shift = segment_shift + 2, items = sel.groups << shift;       // a segment has 4 vectors of each of its steps
+    static_assert(UNROLL == 4, "");
     for (int i0 = tid; i0 < items; i0 += AHEAD * THREADS) {
         uint4 v[AHEAD];
         int at[AHEAD];
@@ -744,12 +745,12 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
             const int i = i0 + a * THREADS;
             at[a] = -1;
             if (i >= items) continue;
-            const int chosen = sel.chosen[i / per], q = i % per, segment = chosen / THREADS, t = chosen % THREADS;
+            const int chosen = sel.chosen[i >> shift], q = i & ((1 << shift) - 1), segment = chosen / THREADS, t = chosen % THREADS;
             if (segment == SEGMENTS) {                  // the parts at the row's ends
                 if (q == 0 && t == 0 && sl.head) at[a] = 0;
                 if (q == 0 && t == 1 && sl.tail) at[a] = sl.nv - 1;
             } else {
-                const int j = sl.full0 + (segment * segment_steps + q / UNROLL) * (THREADS * UNROLL) + (t >> 5) * WARP_STEP +
+                const int j = sl.full0 + ((segment << segment_shift) + q / UNROLL) * (THREADS * UNROLL) + (t >> 5) * WARP_STEP +
                               q % UNROLL * 32 + (t & 31);
                 if (j < sl.full1) at[a] = j;
             }
@@ -807,8 +808,9 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
     Selection& sel = *reinterpret_cast<Selection*>(vocab_smem);
     float* group = group_;
     const int tid = threadIdx.x;
-    const long long r = blockIdx.x / static_cast<unsigned>(p.splits);
-    const int rank = blockIdx.x % static_cast<unsigned>(p.splits);
+    const unsigned splits = p.splits, row_index = splits == 1 ? blockIdx.x : blockIdx.x / splits;
+    const long long r = row_index;
+    const int rank = blockIdx.x - row_index * splits;
     const T* row = p.rows.row<T>(r);
     const Slice<T> sl(row, p.rows.V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
@@ -821,12 +823,14 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
         if (tok >= 0 && tok < p.rows.V) x_tok = Elem<T>::f(row[tok]);
     }
     Running<true, NONE> run;
-    const int steps = sl.steps(), segment_steps = (steps + SEGMENTS - 1) / SEGMENTS;
+    const int steps = sl.steps();
+    int segment_shift = 0;              // a segment has 2^segment_shift steps
+    while (steps > SEGMENTS << segment_shift) ++segment_shift;
     if constexpr (TOP)
         for (int i = 0; i < SEGMENTS + 1; ++i) group[i * THREADS + tid] = -INFINITY;
     float largest = -INFINITY;          // of the segment
     float mine = -INFINITY;             // this thread's
-    int left = segment_steps, segment = 0;
+    int left = 1 << segment_shift, segment = 0;
     ring.stream([](int, uint32_t) {}, [&](int step, uint4 (&v)[UNROLL], bool whole) {
         if constexpr (!TOP) {
             run.template add<T>(v, whole, [&] { return max_of<T>(v); }, c, 0.f);
@@ -838,7 +842,7 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
                 group[segment * THREADS + tid] = largest;
                 mine = max_nan(mine, largest);
                 ++segment;
-                left = segment_steps;
+                left = 1 << segment_shift;
                 largest = -INFINITY;
             }
         }
@@ -871,7 +875,7 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
     };
     if (p.splits == 1 && tid == THREADS - 1) finish();
     int n = 0;
-    if constexpr (TOP) n = select_best<T>(sel, group, sl, p.k, mine, segment_steps);
+    if constexpr (TOP) n = select_best<T>(sel, group, sl, p.k, mine, segment_shift);
 
     if (p.splits > 1) {
         if (tid == 0) {
@@ -1141,8 +1145,9 @@ __global__ void __launch_bounds__(THREADS, 3) topk_distillation_kernel(const __g
     __shared__ double part_of[MAX_K / 32][4];
     __shared__ float list_max[2][MAX_K / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long r = blockIdx.x / static_cast<unsigned>(p.splits);
-    const int rank = blockIdx.x % static_cast<unsigned>(p.splits);
+    const unsigned splits = p.splits, row_index = splits == 1 ? blockIdx.x : blockIdx.x / splits;
+    const long long r = row_index;
+    const int rank = blockIdx.x - row_index * splits;
     const int V = p.rows.V;
     const T* row = p.rows.row<T>(r);
     const Slice<T> sl(row, V, rank, p.splits);
