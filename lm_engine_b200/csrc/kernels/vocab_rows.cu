@@ -3,12 +3,17 @@
 //
 // With y = x / temperature, m the row's largest logit and t_j = (x_j - m) / temperature, everything that a row needs is
 //   S = sum exp(t_j),   W = sum exp(t_j) t_j,   log p_j = t_j - log S,   entropy = log S - W / S
-// and a handful of single logits.  The exponent is taken after the subtraction, so no large numbers meet in it, whatever
-// the temperature; sums run in fp32 per thread and are joined in 64 bits, where the few values per row are finished too.
+// and a handful of single logits.  The exponent is a difference taken in one rounding or before the product, so no large
+// numbers meet in it, whatever the temperature; sums run in fp32 per thread and are joined in 64 bits, where the few values
+// per row are finished too.
 //
-// Bound by HBM (one read of the logits forward, a read and a write backward): a CTA of 256 threads streams a row, or its
-// part of a row, with 16-byte loads and a running maximum per thread; rows are split over a cluster of up to 8 CTAs when
-// there are few of them, and joined through distributed shared memory: one launch, no workspace, a fixed order of sums.
+// Bound by HBM (one read of the logits forward, a read and a write backward) and, sustained, by the power that the
+// instructions per logit take: a CTA of 256 threads streams a row through rings of bulk copies, one per warp; rows are split
+// over a cluster of up to 8 CTAs when there are few of them, and joined through distributed shared memory: one launch, no
+// workspace, a fixed order of sums.
+// Measured on a B200 (1000 W, sustained): scores of 4094 x 128256 bf16 logits 171 us = 6.1 TB/s, with the best 64 of 4096
+// rows 220 us = 4.8 TB/s (selection: 12 of the 42 thousand cycles of a row); gradient at 4096 x 128256 327 us = 6.4 TB/s;
+// distillation at 8192 x 128256 with the best 64, forward 348 us = 6.0 TB/s, backward 648 us = 6.5 TB/s.
 // Included by lme_cuda.cu after decode_attention.cu.
 #include <cuda_fp16.h>
 
@@ -360,55 +365,85 @@ constexpr float TRY_BELOW = 1.2676506e30f;              // 2^100
 enum AtOne { NONE, OWN, SQUARE };
 template <bool ENTROPY, AtOne ONE>
 struct Running {
-    float m = -INFINITY, limit = -INFINITY, s = 0.f, w = 0.f, s1 = 0.f;    // s1: s at temperature one (c1)
+    float m = -INFINITY, limit = -INFINITY;
+    // s and w, and what their additions have lost.  Vectors, then steps are added up by themselves: next to a token that the model
+    // is sure of, single small terms would be lost in its thread's sums, all of them downwards (entropies of 128256 logits at
+    // temperature 0.8: off by 1.1e-5 on average, so by 2e-7; 2 to 3 % of the time).
+    float s = 0.f, w = 0.f, s_lost = 0.f, w_lost = 0.f;
+    float s1 = 0.f;                 // s at temperature one (c1)
     bool far = false;               // LOW is so far below the base that it counts nothing
     bool trying = false, tried = false;
     float n = 0.f, n1 = 0.f;        // while trying
 
+    // to another unit, 2^by times smaller
+    __device__ __forceinline__ void change(float by, float f) {
+        if (ENTROPY) {
+            w = (w + s * by) * f;
+            w_lost = (w_lost + s_lost * by) * f;
+        }
+        s *= f;
+        s_lost *= f;
+    }
     __device__ __forceinline__ void raise(float to, float c, float c1) {
         const float d = m - to;
         const float t = max_nan(d * c, T_MIN);          // (-inf) - (-inf) cannot be: `to` is above m
-        const float f = exp2_approx(t);
-        if (ENTROPY) w = (w + s * t) * f;
-        s *= f;
+        change(t, exp2_approx(t));
         if (ONE) s1 *= exp2_approx(max_nan(d * c1, T_MIN));
         m = to;
         limit = to + __fdividef(SLACK, ONE ? fmaxf(c, c1) : c);
     }
-    // from units of 2^(m c) to those of 2^n and back
-    __device__ __forceinline__ void change(float by, float by1) {
-        const float f = exp2_approx(by);
-        if (ENTROPY) w = (w + s * by) * f;
-        s *= f;
-        if (ONE == SQUARE) s1 *= f * f;
-        if (ONE == OWN) s1 *= exp2_approx(by1);
-    }
+    // from units of 2^(m c) to those of 2^n
     __device__ __forceinline__ void enter(float c, float c1) {
         if (m == -INFINITY) return;                     // (no base yet)
         tried = true;
         if (!(fabsf(m) * (ONE == OWN ? fmaxf(c, c1) : c) < 1e6f)) return;
         n = rintf(m * c);
-        n1 = ONE == OWN ? rintf(m * c1) : 0.f;
-        change(fmaf(m, c, -n), fmaf(m, c1, -n1));
+        const float by = fmaf(m, c, -n), f = exp2_approx(by);
+        change(by, f);
+        if (ONE == SQUARE) s1 *= f * f;
+        if (ONE == OWN) {
+            n1 = rintf(m * c1);
+            s1 *= exp2_approx(fmaf(m, c1, -n1));
+        }
         trying = true;
     }
     __device__ __forceinline__ void leave(float c, float c1) {
         if (!trying) return;
-        change(-fmaf(m, c, -n), -fmaf(m, c1, -n1));
+        const float by = -fmaf(m, c, -n), f = exp2_approx(by);
+        change(by, f);
+        if (ONE == SQUARE) s1 *= f * f;
+        if (ONE == OWN) s1 *= exp2_approx(-fmaf(m, c1, -n1));
+        trying = false;
+    }
+    // At the end, for entropies: the base moves to where the thread's sum is about one, before w is rounded to what is left of
+    // it.  In 64 bits: the two terms of the new w are much larger than it.
+    __device__ __forceinline__ void settle(float c) {
+        if (!(s > 0.f && s < INFINITY)) {
+            leave(c, 0.f);
+            return;
+        }
+        float l;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(l) : "f"(s));
+        l = rintf(l);
+        const float to = trying ? __fdividef(n + l, c) : m + __fdividef(l, c);
+        const float by = trying ? fmaf(to, c, -(n + l)) : fmaf(to - m, c, -l);      // beside the power of two
+        if (!(fabsf(by) < 1.f)) {                       // (bases too large for such steps)
+            leave(c, 0.f);
+            return;
+        }
+        const double s_ = static_cast<double>(s) - s_lost, w_ = static_cast<double>(w) - w_lost;
+        const double f = exp2_approx(-by) * __int_as_float((127 - static_cast<int>(fmaxf(fminf(l, 120.f), -120.f))) << 23);
+        w = static_cast<float>((w_ - s_ * (static_cast<double>(l) + by)) * f);
+        s = static_cast<float>(s_ * f);
+        s_lost = w_lost = 0.f;
+        m = to;
         trying = false;
     }
     // whole: no vector of the step is filled up; largest(): of the step
     template <typename T, int U, typename F>
     __device__ __forceinline__ void add(const uint4 (&r)[U], bool whole, F&& largest, float c, float c1) {
         if (trying) {
-            if (whole) {
-                const float s_ = s, w_ = w, s1_ = s1;
-                sum<T, U, true, false, false>(r, c, c1);
-                if (s < TRY_BELOW && (!ENTROPY || fabsf(w) < INFINITY) && (!ONE || s1 < TRY_BELOW)) return;
-                s = s_;
-                w = w_;
-                s1 = s1_;
-            }
+            if (whole && sum<T, U, true, false, false>(r, c, c1)) return;
             leave(c, c1);
         }
         const float x = largest();
@@ -423,12 +458,13 @@ struct Running {
         else sum<T, U, false, false, true>(r, c, c1);
         if (!tried) enter(c, c1);
     }
+    // false, and nothing added, where a try has run over
     template <typename T, int U, bool TRY, bool LIMIT_X, bool LIMIT_T>
-    __device__ __forceinline__ void sum(const uint4 (&r)[U], float c, float c1) {
+    __device__ __forceinline__ bool sum(const uint4 (&r)[U], float c, float c1) {
         constexpr int N = Elem<T>::N;
         const float base = TRY ? n : m == -INFINITY ? 0.f : m;
         const unsigned long long nb = pair(-base, -base), nb1 = pair(-n1, -n1), cc = pair(c, c), cc1 = pair(c1, c1);
-        unsigned long long s2 = pair(s, 0.f), w2 = pair(w, 0.f), s12 = pair(s1, 0.f);
+        unsigned long long s2 = 0, w2 = 0, s12 = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             uint4 v = r[u];
@@ -438,6 +474,7 @@ struct Running {
             }
             float f[N];
             Elem<T>::unpack(v, f);
+            unsigned long long sv = 0, wv = 0;          // of the vector
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
                 const unsigned long long x = pair(f[e], f[e + 1]), d = TRY ? x : add2(x, nb);
@@ -447,19 +484,34 @@ struct Running {
                     t.y = max_nan(t.y, T_MIN);
                 }
                 const unsigned long long q = pair(exp2_approx(t.x), exp2_approx(t.y));
-                s2 = add2(s2, q);
-                if (ENTROPY) w2 = fma2(q, pair(t.x, t.y), w2);
+                sv = e == 0 ? q : add2(sv, q);
+                if (ENTROPY) wv = e == 0 ? mul2(q, pair(t.x, t.y)) : fma2(q, pair(t.x, t.y), wv);
                 if (ONE == SQUARE) s12 = fma2(q, q, s12);
                 if (ONE == OWN) {
                     const float2 t1 = halves(TRY ? fma2(x, cc1, nb1) : mul2(d, cc1));
                     s12 = add2(s12, pair(exp2_approx(t1.x), exp2_approx(t1.y)));
                 }
             }
+            s2 = u == 0 ? sv : add2(s2, sv);
+            if (ENTROPY) w2 = u == 0 ? wv : add2(w2, wv);
         }
         const float2 a = halves(s2), b = halves(w2), a1 = halves(s12);
-        s = a.x + a.y;
-        if (ENTROPY) w = b.x + b.y;
-        if (ONE) s1 = a1.x + a1.y;
+        const float ds = a.x + a.y, dw = b.x + b.y, ds1 = a1.x + a1.y;
+        if (TRY && !(ds < TRY_BELOW && (!ENTROPY || fabsf(dw) < INFINITY) && (!ONE || ds1 < TRY_BELOW))) return false;
+        if (ONE) s1 += ds1;
+        if (!ENTROPY) {
+            s += ds;
+            return true;
+        }
+        // compensated, both at once
+        const unsigned long long minus = pair(-1.f, -1.f), old = pair(s, w), y = fma2(pair(s_lost, w_lost), minus, pair(ds, dw));
+        const unsigned long long sum = add2(old, y), lost = fma2(y, minus, fma2(old, minus, sum));
+        const float2 now = halves(sum), gone = halves(lost);
+        s = now.x;
+        s_lost = gone.x;
+        w = now.y;
+        w_lost = gone.y;
+        return true;
     }
 };
 // The CTA's sums, relative to its largest base, in every thread (`red`: 4 * WARPS floats).
@@ -469,7 +521,8 @@ struct Sums {
 };
 template <bool ENTROPY, AtOne ONE>
 __device__ __forceinline__ Sums join_block(Running<ENTROPY, ONE> r, float c, float c1, float* red) {
-    r.leave(c, c1);
+    if (ENTROPY) r.settle(c);
+    else r.leave(c, c1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float m = r.m;
 #pragma unroll
@@ -479,7 +532,7 @@ __device__ __forceinline__ Sums join_block(Running<ENTROPY, ONE> r, float c, flo
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) m = max_nan(m, red[i]);
     if (!(m <= r.m)) r.raise(m, c, c1);
-    const float s = warp_sum(r.s), w = ENTROPY ? warp_sum(r.w) : 0.f, s1 = ONE ? warp_sum(r.s1) : 0.f;
+    const float s = warp_sum(r.s - r.s_lost), w = ENTROPY ? warp_sum(r.w - r.w_lost) : 0.f, s1 = ONE ? warp_sum(r.s1) : 0.f;
     if (lane == 0) {
         red[WARPS + warp] = s;
         red[2 * WARPS + warp] = w;
@@ -797,6 +850,8 @@ struct ScoreArgs {
     float* stats;                   // [rows][4]: m, S, entropy, log S; or null
 };
 
+// Three CTAs per SM with 80 registers: with four and 64 the tried steps take 13 % more instructions (4094 x 128256 bf16,
+// sustained: 186 and 191 us; with the best 64: 233 and 249).
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid_constant__ ScoreArgs p) {
     __shared__ float red[4 * WARPS];
@@ -1134,8 +1189,10 @@ struct DistillPart {        // of a CTA, relative to its largest logit m
     double px;              // METHOD 1: sum of listed exponentials times (x / temperature - teacher's log)
 };
 
+// Four CTAs per SM: there is more to do around a row's stream than above, which the others hide (2047 x 50257 bf16: 48 us, 53
+// with three and more registers; 8192 x 128256: 366 and 364).
 template <typename T, AtOne ONE>
-__global__ void __launch_bounds__(THREADS, 3) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
+__global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
     constexpr int N = Elem<T>::N;
     extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then a byte per vector of this CTA
     uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + ring_bytes(p.stages));
@@ -1457,18 +1514,21 @@ inline cudaError_t launch(Kern kern, const Args& a, long long ctas, int splits, 
 }
 
 inline int elem_size(int dtype) { return dtype == LME_F32 ? 4 : 2; }
-// Steps of a gradient's CTA: four, so that what it has to know of its row costs little, fewer where that would leave SMs
-// idle.
+// Steps of a gradient's CTA: eight where that still makes many CTAs, so that what it has to know of its row costs little, else
+// four, fewer where SMs would be idle.  Distillation at 8192 x 128256 bf16, backward: 656 us with eight, 668 with four, 741
+// with two; at 2047 x 50257: 82 with eight, 77 with four, 86 with two.
 struct GradGrid {
     int chunks, steps;
 };
 inline GradGrid grad_grid(long long rows, int V, int elem) {
     const int n = 16 / elem, step = THREADS * UNROLL;
     const int vectors = static_cast<int>((V + 2ll * n - 2) / n), all = (vectors + step - 1) / step;   // the first may be a part
-    int steps = 4;
-    while (steps > 1 && rows * ((all + steps - 1) / steps) < 148 * 8) steps /= 2;
-    return {(all + steps - 1) / steps, steps};
+    auto chunks = [&](int steps) { return (all + steps - 1) / steps; };
+    int steps = rows * chunks(8) >= 148 * 40 ? 8 : 4;
+    while (steps > 1 && rows * chunks(steps) < 148 * 8) steps /= 2;
+    return {chunks(steps), steps};
 }
+
 // Dynamic shared memory of the streaming kernels; the attribute is set to the most that any call asks for.
 constexpr int RING_STAGES = 2;
 constexpr int MAX_SMEM = ring_bytes(RING_STAGES) + MAX_MAP;

@@ -173,17 +173,20 @@ _len_torch_dispatch_stack = torch._C._len_torch_dispatch_stack
 _peek_interpreter_stack = torch._C._functorch.peek_interpreter_stack
 
 
-def eager(*tensors: torch.Tensor) -> bool:
+def eager(*tensors: torch.Tensor | None) -> bool:
     """Whether kernels may take these tensors by address: plain tensors of the current device, outside tracing,
     functorch transforms, forward-mode AD and dispatch modes, all of which need operations that they can see."""
     if (torch.compiler.is_compiling() or _is_tracing() or _len_torch_dispatch_stack()
             or torch.autograd.forward_ad._current_level >= 0 or _peek_interpreter_stack() is not None):
         return False
+    device = None
     for t in tensors:
+        if t is None:
+            continue
         if (type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda:
             return False
-    device = torch._C._cuda_getDevice()
-    for t in tensors:
+        if device is None:
+            device = torch._C._cuda_getDevice()
         if t.get_device() != device:
             return False
     return True

@@ -50,7 +50,7 @@ def logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     are, or the vocabulary is not dense."""
     V = x.size(-1)
     if x.is_contiguous():
-        return x, max(x.numel() // V, 1), V, 0
+        return x, x.numel() // V or 1, V, 0
     levels: list[tuple[int, int]] = []          # (size, stride) from the inside, dimensions of size 1 left out
     for d in range(x.dim() - 2, -1, -1):
         size, stride = x.size(d), x.stride(d)
@@ -71,11 +71,11 @@ def kernel_usable(logits: torch.Tensor, temperature, *others: torch.Tensor | Non
     """A temperature that is a tensor may want a gradient: it is left to the PyTorch operations."""
     if logits.dtype not in KERNEL_TYPES or isinstance(temperature, torch.Tensor) or logits.size(-1) > 1 << 30:
         return False
-    return _lib.eager(logits, *[t for t in others if t is not None])
+    return _lib.eager(logits, *others)
 
 
 def check_logits(logits: torch.Tensor, temperature) -> None:
-    if logits.dim() == 0 or logits.size(-1) == 0 or not logits.is_floating_point():
+    if logits.dim() == 0 or logits.size(-1) == 0 or (logits.dtype not in KERNEL_TYPES and not logits.is_floating_point()):
         raise ValueError(f"logits need a floating type and a vocabulary, got {logits.dtype} of {tuple(logits.shape)}")
     if not isinstance(temperature, torch.Tensor) and not 0 < temperature < float("inf"):
         raise ValueError(f"temperature has to be positive, got {temperature}")
@@ -173,7 +173,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     check_logits(logits, temperature)
     if tokens is not None:
         check_tokens("tokens", tokens, logits)
-    if not 0 <= top_k <= min(MAX_TOP_K, logits.size(-1)):
+    if top_k and not 0 < top_k <= min(MAX_TOP_K, logits.size(-1)):
         raise ValueError(f"top_k has to be in 0..{min(MAX_TOP_K, logits.size(-1))}, got {top_k}")
     if not kernel_usable(logits, temperature, tokens):
         return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)
