@@ -594,6 +594,7 @@ struct Selection {
     int bin[BINS];
     uint32_t hi[WARPS], lo[WARPS];
     float reach;
+    int pick, above, through, crowded;
     int groups, count, scan[WARPS];
 };
 
@@ -718,18 +719,52 @@ __device__ __noinline__ int select_by_passes(Selection& sel, const Slice<T>& sl,
     return min(have, k);
 }
 
+// The bin in which the need-th from above falls (sel.pick, -1 if there are fewer), and how many are above it.  First warp.
+__device__ __forceinline__ void pick_bin(Selection& sel, int need) {
+    constexpr int PER = BINS / 32;
+    const int lane = threadIdx.x & 31;
+    int n[PER], mine = 0;                               // lane 0 has the uppermost bins
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += n[i] = sel.bin[BINS - 1 - (lane * PER + i)];
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int above = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += above;
+    }
+    const uint32_t enough = __ballot_sync(0xffffffffu, upto >= need);
+    if (enough == 0) {
+        if (lane == 0) sel.pick = -1;
+    } else if (lane == __ffs(enough) - 1) {
+        int at = BINS, have = upto - mine, above = have;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (have < need) {
+                above = have;
+                have += n[i];
+                at = BINS - 1 - (lane * PER + i);
+            }
+        sel.pick = at;
+        sel.above = above;
+        sel.through = have;
+    }
+}
+
 // A value that at least k of the threads' largest values reach and hardly more do, into sel.reach: the edge of the bin of a
-// histogram in which the k-th falls.  NaN, which compares as reached, where there is no such value or the histogram finds none.
+// histogram in which the k-th falls.  Where too many fall into it (values of masked vocabularies or outliers stretch the bins,
+// values are equal) the k-th is found by the bits of its key, eight at a time.  NaN, which compares as reached, where fewer than k
+// threads have anything.
 __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool finite = largest > -INFINITY;            // (no vectors, or nothing but -inf: not counted)
+    const bool some = !(largest == -INFINITY);          // (no vectors, or nothing but -inf: not counted)
     const uint32_t key = key_of(largest);
-    const uint32_t hi = __reduce_max_sync(0xffffffffu, key), lo = __reduce_min_sync(0xffffffffu, finite ? key : 0xffffffffu);
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, key), lo = __reduce_min_sync(0xffffffffu, some ? key : 0xffffffffu);
     if (lane == 0) {
         sel.hi[warp] = hi;
         sel.lo[warp] = lo;
     }
-    for (int i = tid; i < BINS; i += THREADS) sel.bin[i] = 0;
+    static_assert(BINS == THREADS, "");
+    sel.bin[tid] = 0;
     __syncthreads();
     uint32_t top = 0, bottom = 0xffffffffu;
 #pragma unroll
@@ -738,36 +773,36 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
         bottom = min(bottom, sel.lo[i]);
     }
     const float from = value_of(bottom), scale = __fdividef(BINS - 0.01f, value_of(top) - from);    // (0 or NaN: one bin)
-    if (finite) atomicAdd(&sel.bin[min(BINS - 1, max(0, static_cast<int>((largest - from) * scale)))], 1);
+    if (some) atomicAdd(&sel.bin[min(BINS - 1, max(0, static_cast<int>((largest - from) * scale)))], 1);
     __syncthreads();
     if (warp == 0) {
-        constexpr int PER = BINS / 32;
-        int n[PER], mine = 0;                           // lane 0 has the uppermost bins
-#pragma unroll
-        for (int i = 0; i < PER; ++i) mine += n[i] = sel.bin[BINS - 1 - (lane * PER + i)];
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int above = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += above;
-        }
-        const uint32_t enough = __ballot_sync(0xffffffffu, upto >= k);
-        if (enough == 0) {
-            if (lane == 0) sel.reach = __int_as_float(0x7fffffff);
-        } else if (lane == __ffs(enough) - 1) {
-            int b = BINS - 1 - lane * PER, have = upto - mine;
-#pragma unroll
-            for (int i = 0; i < PER - 1; ++i) {
-                have += n[i];
-                if (have < k) --b;
-                else have = k;
-            }
+        pick_bin(sel, k);
+        __syncwarp();
+        if (lane == 0) {
             // below the bin's edge by more than the roundings of where its values are
-            sel.reach = from + static_cast<float>(b) / scale - (fabsf(from) + fabsf(value_of(top))) * 2e-6f;
+            const float edge = from + static_cast<float>(sel.pick) / scale - (fabsf(from) + fabsf(value_of(top))) * 2e-6f;
+            sel.reach = sel.pick < 0 ? __int_as_float(0x7fffffff) : edge;
+            sel.crowded = sel.pick >= 0 && (sel.through > 2 * k + 64 || edge != edge);
+            sel.groups = sel.count = 0;
         }
-        if (lane == 0) sel.groups = sel.count = 0;
     }
     __syncthreads();
+    if (sel.crowded) {
+        uint32_t prefix = 0;
+        int need = k;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            sel.bin[tid] = 0;
+            __syncthreads();
+            if (some && (shift == 24 || key >> (shift + 8) == prefix)) atomicAdd(&sel.bin[key >> shift & 255], 1);
+            __syncthreads();
+            if (warp == 0) pick_bin(sel, need);
+            __syncthreads();
+            prefix = prefix << 8 | static_cast<uint32_t>(sel.pick);
+            need -= sel.above;
+        }
+        if (tid == 0) sel.reach = value_of(prefix);
+        __syncthreads();
+    }
 }
 
 // The k best of a slice, in order, into sel.best; returns how many the slice has.  The stream has left each thread's largest

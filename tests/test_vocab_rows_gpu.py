@@ -597,3 +597,34 @@ def test_distillation_wrapper(method):
     assert abs(float(out["lm_loss"]) - float(want.nll.mean())) < e
     assert all(p.grad is not None and torch.isfinite(p.grad.float()).all() for p in w.model.parameters())
     assert all(p.grad is None for p in w.teacher_model.parameters()) and _lib.read_status()[0] == 0
+
+
+@pytest.mark.parametrize("rows", [1, 450])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("V", [3001, 40001])
+def test_alternatives_beside_outliers_and_masks(rows, dtype, V):
+    """Values that stretch the range of a row's largest ones: masks by the type's lowest, outliers, both infinities."""
+    x = _rows(1, rows, V, dtype, 21)
+    low = torch.finfo(dtype).min
+    for k in (1, 20, 128):
+        y = x.clone()
+        y[..., V // 3:] = low
+        _score(y, None, k, 1.0, grads=False)
+        y = x.clone()
+        y[..., : V - 200] = low
+        _score(y, None, k, 1.0, grads=False)
+        y = x.clone()
+        y[..., V // 2] = 30000.0
+        y[..., V // 5] = -30000.0
+        _score(y, None, k, 1.0, grads=False)
+        y = torch.where(torch.arange(V, device="cuda") % 17 == 3, x, torch.tensor(low, device="cuda").to(dtype))
+        _score(y, None, k, 1.0, grads=False)
+        y = x * 0 - 5
+        y[..., 7::50] = -4.0
+        y[..., 8::50] = 3.0
+        _score(y, None, k, 1.0, grads=False)
+        y = x.clone()
+        y[..., V // 7] = math.inf
+        y[..., V // 3] = math.nan
+        y[..., 2 * V // 3] = -math.inf
+        _score(y, None, k, 1.0, grads=False)
