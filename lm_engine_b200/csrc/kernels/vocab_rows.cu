@@ -599,7 +599,7 @@ struct Selection {
 };
 
 // The first k of the n candidates, in order, into `best`; returns how many there are.  All threads.
-__device__ __noinline__ int order_candidates(Selection& sel, int n, int k) {
+__device__ __forceinline__ int order_candidates(Selection& sel, int n, int k) {
     const int tid = threadIdx.x;
     if (n <= THREADS) {             // the place of a candidate is the number of those ahead of it: some lanes count for each
         const int shift = n <= THREADS / 8 ? 3 : n <= THREADS / 4 ? 2 : n <= THREADS / 2 ? 1 : 0, lanes = 1 << shift;
@@ -635,9 +635,11 @@ __device__ __noinline__ int order_candidates(Selection& sel, int n, int k) {
 
 // Rows with so many values at or above the first bound that they do not fit (constant rows, above all): the k-th key bit
 // by bit with a pass over the slice for each, then those above it, then the first of those equal to it.
+// (What is out of line makes its slice anew: one passed by reference would live in memory all the while.)
 template <typename T>
-__device__ __noinline__ int select_by_passes(Selection& sel, const Slice<T>& sl, int k) {
+__device__ __noinline__ int select_by_passes(Selection& sel, const T* row, int V, int rank, int splits, int k) {
     constexpr int N = Elem<T>::N;
+    const Slice<T> sl(row, V, rank, splits);
     const int tid = threadIdx.x;
     uint32_t bound = 0;
     bool exact = false;
@@ -810,8 +812,10 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
 // hardly more (1.2 k for k = 64 where values come in no order), so only the segments that do are read again.  Few
 // instructions matter more than few reads: the other CTAs of the SM stream meanwhile, and a warp gets every eighth slot.
 template <typename T>
-__device__ __noinline__ int select_best(Selection& sel, const float* group, const Slice<T>& sl, int k, float largest, int segment_shift) {
+__device__ __noinline__ int select_best(Selection& sel, const float* group, const T* row, int V, int rank, int splits, int k,
+                                        float largest, int segment_shift) {
     constexpr int N = Elem<T>::N, AHEAD = 4;
+    const Slice<T> sl(row, V, rank, splits);
     const int tid = threadIdx.x;
     find_reach(sel, largest, k);
     const float reach = sel.reach;
@@ -868,7 +872,7 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
     }
     __syncthreads();
     int n = sel.count;
-    if (n > MAX_CANDIDATES) n = select_by_passes<T>(sel, sl, k);
+    if (n > MAX_CANDIDATES) n = select_by_passes<T>(sel, row, V, rank, splits, k);
     __syncthreads();
     return min(order_candidates(sel, n, k), sl.size());
 }
@@ -965,7 +969,7 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
     };
     if (p.splits == 1 && tid == THREADS - 1) finish();
     int n = 0;
-    if constexpr (TOP) n = select_best<T>(sel, group, sl, p.k, mine, segment_shift);
+    if constexpr (TOP) n = select_best<T>(sel, group, row, p.rows.V, rank, p.splits, p.k, mine, segment_shift);
 
     if (p.splits > 1) {
         if (tid == 0) {
