@@ -1217,7 +1217,7 @@ struct DistillArgs {
     int* entries;                   // [rows][k]: the ids that count, -1 elsewhere
     float* stats;                   // [rows][8]
 };
-// stats: m, 1 / S, factor of p_j at tokens that are not listed, sum q + q_r (METHOD 0) or the loss (METHOD 1), what is taken
+// stats: the base m of the gradient's exponentials, 1 / S, factor of p_j at tokens that are not listed, sum q + q_r (METHOD 0) or the loss (METHOD 1), what is taken
 // from the teacher's values to make them log probabilities, 1 / S at temperature one, log S, 1 if the row has any loss
 
 struct DistillPart {        // of a CTA, relative to its largest logit m
@@ -1448,9 +1448,15 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
                 p.nll[r] = !labelled              ? 0.f
                            : label >= 0 && label < V ? static_cast<float>(log_s1 - (static_cast<double>(x_label) - all.m))
                                                      : __int_as_float(0x7fffffff);
+            // The gradient's exponentials are relative to where the sums are about one (both of them at least one), so that the
+            // logarithms that it subtracts are small.
+            double up = log_s / p.inv_temperature;
+            if (ONE) up = fmin(up, log_s1);
+            const float m2 = static_cast<float>(all.m + up);
+            const double moved = static_cast<double>(m2) - all.m, log_s2 = log_s - moved * p.inv_temperature;
             float4* st = reinterpret_cast<float4*>(p.stats + 8 * r);
-            st[0] = make_float4(all.m, static_cast<float>(1 / S), static_cast<float>(factor), static_cast<float>(fourth));
-            st[1] = make_float4(static_cast<float>(norm), static_cast<float>(1 / S1), static_cast<float>(log_s), 1.f);
+            st[0] = make_float4(m2, static_cast<float>(exp(-log_s2)), static_cast<float>(factor), static_cast<float>(fourth));
+            st[1] = make_float4(static_cast<float>(norm), static_cast<float>(exp(moved - log_s1)), static_cast<float>(log_s2), 1.f);
         }
     }
     if (p.splits > 1) cluster_sync();

@@ -19,6 +19,8 @@ from .logprobs import KERNEL_TYPES, MAX_TOP_K, as_int64, check_logits, check_tok
 #: The teacher's mass outside of its listed tokens is one minus their sum, which the rounding of fp32 log probabilities moves by
 #: about this much: a smaller rest counts as none, and as this much where its logarithm is asked for.
 NO_TAIL = 2.0 ** -20
+#: The kernel keeps a bit per logit in shared memory; beyond this the PyTorch operations serve.
+MAX_KERNEL_VOCAB = 3_000_000
 
 
 class TopkDistillation(NamedTuple):
@@ -164,7 +166,7 @@ def topk_distillation(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs:
                          f"{tuple(top_logprobs.shape)}")
     if labels is not None:
         check_tokens("labels", labels, logits)
-    if not kernel_usable(logits, temperature, top_ids, top_logprobs, labels):
+    if logits.size(-1) > MAX_KERNEL_VOCAB or not kernel_usable(logits, temperature, top_ids, top_logprobs, labels):
         return topk_distillation_reference(logits, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index)
     if labels is not None:
         labels = as_int64(labels)

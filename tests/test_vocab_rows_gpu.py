@@ -628,3 +628,37 @@ def test_alternatives_beside_outliers_and_masks(rows, dtype, V):
         y[..., V // 3] = math.nan
         y[..., 2 * V // 3] = -math.inf
         _score(y, None, k, 1.0, grads=False)
+
+
+def test_distillation_of_no_rows_and_of_long_rows():
+    from lm_engine_b200.ops import topk_distillation
+
+    x = _rows(1, 4, 300, BF, 1).requires_grad_(True)
+    ids, lq = _lists(x.detach(), 4, 1)
+    out = topk_distillation(x[:, :0], ids[:, :0], lq[:, :0], ids[:, :0, 0])
+    assert out.kl_divergence.shape == out.nll.shape == (1, 0)
+    (g,) = torch.autograd.grad(out.kl_divergence.sum() + out.nll.sum(), x)
+    assert float(g.abs().max()) == 0
+    x = _rows(1, 2, 1_200_003, BF, 1)
+    ids, lq = _lists(x, 100, 1)
+    _distill(x, ids, lq, ids[..., 7], "backward", True, 1.0)
+    _score(x, ids[..., 3], 100, 1.0)
+
+
+@pytest.mark.parametrize("offset", [0.0, 100.0])
+def test_fp32_gradients_of_the_forward_divergence_are_fp32(offset):
+    """Logits whose largest come late in a row, far above a thread's first: the gradient subtracts logarithms."""
+    from lm_engine_b200.ops import topk_distillation, topk_distillation_reference
+
+    x = _rows(1, 300, 20000, F32, 8) * 0.5
+    x[..., 15000:] += 30.0
+    x = (x + offset).requires_grad_(True)
+    ids, lq = _lists(x.detach(), 20, 4)
+    x64 = x.detach().double().requires_grad_(True)
+    for temperature in (1.0, 2.0, 0.7):
+        (got,) = torch.autograd.grad(topk_distillation(x, ids, lq, ids[..., 0], "forward", True, temperature)
+                                     .kl_divergence.sum(), x)
+        (ref,) = torch.autograd.grad(topk_distillation_reference(x64, ids, lq, ids[..., 0], "forward", True, temperature)
+                                     .kl_divergence.sum(), x64)
+        # p (log p - log q - KL): logarithms of at most 2^5, a few roundings of 2^-24 each, of terms that partly cancel
+        assert float((got.double() - ref).norm() / ref.norm()) < 2.0 ** -24 * 2 ** 5 * 4
