@@ -27,8 +27,8 @@ constexpr int WARP_STEP = 32 * UNROLL;  // vectors of a warp and step
 constexpr int MAX_SPLITS = 8;           // CTAs of a cluster
 constexpr int MAX_K = LME_VOCAB_MAX_K;  // best tokens, or tokens of a teacher, per row
 constexpr int SEGMENTS = 8;             // of a CTA's steps: what the selection reads again goes by their maxima
-constexpr int MAX_CANDIDATES = 2048;
-constexpr int MAX_MAP = 96 * 1024;      // bytes of the map of listed tokens: a byte per vector of a CTA
+constexpr int MAX_CANDIDATES = 1024;
+constexpr int MAX_MAP = 96 * 1024;      // bytes of the map of listed tokens, a byte for each vector of a CTA
 constexpr float T_MIN = -150.f;         // 2^-150 is zero here; keeps 0 * (-inf) out of the sums
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr double LN2 = 0.6931471805599453;
@@ -283,9 +283,9 @@ struct Ring {
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(address) : "memory");
         return r;
     }
-    // f(step, vectors, whether all of them are there) for every step; nothing behind the last whole vector.  After a wait that ran out the loop goes on
+    // f(step, vectors, whether all of them are there) for every step; nothing behind the last whole vector.  first(step,
+    // address): before a lane reads its vectors, 512 bytes apart from `address` on.  After a wait that ran out the loop goes on
     // without waiting (wrong rows, status word set).
-    // first(step, address): before a lane reads its vectors, 512 bytes apart from `address` on.
     template <typename F0, typename F>
     __device__ __forceinline__ void stream(F0&& first, F&& f) {
         const int lane = threadIdx.x & 31;
@@ -359,7 +359,7 @@ __host__ __device__ constexpr int ring_bytes(int stages) { return WARPS * stages
 // over or are NaN the step is done again in the careful way, and the rest of the row too.
 constexpr float SLACK = 8.f;
 constexpr float TRY_BELOW = 1.2676506e30f;              // 2^100
-// AT_ONE: how the sum at temperature one is found beside the other: not at all, by exponentials of its own (as many again, and the
+// AtOne: how the sum at temperature one is found beside the other: not at all, by exponentials of its own (as many again, and the
 // exponential unit is what bounds the stream then), or at temperature two by squares.  Distillation of 4096 x 128256
 // bf16 logits at temperature two, forward: 277 us with exponentials of their own, 205 with squares.
 enum AtOne { NONE, OWN, SQUARE };
@@ -865,8 +865,9 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
                 const int b = __ffs(hits) - 1, a = b / N;
                 const int id = sl.index(a == 0 ? at[0] : a == 1 ? at[1] : a == 2 ? at[2] : at[3], b % N);
                 const float x = Elem<T>::f(reinterpret_cast<const T*>(&sel.stash[a][tid])[b % N]);
-                if (to < MAX_CANDIDATES) sel.cand[to] = id >= 0 && id < sl.V ? candidate(key_of(x), id) : 0ull;    // (0: a part's
-                ++to;                                                                                              // other places)
+                // (0 for the places of a part that are not the row's: they come last)
+                if (to < MAX_CANDIDATES) sel.cand[to] = id >= 0 && id < sl.V ? candidate(key_of(x), id) : 0ull;
+                ++to;
             }
         }
     }
@@ -957,7 +958,7 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
         if (p.tokens != nullptr) {
             float lp = 0.f;
             if (tok != p.ignore_index)
-                lp = tok >= 0 && tok < p.rows.V ? static_cast<float>(static_cast<double>(x_tok - sum.m) * p.inv_temperature - log_s)
+                lp = tok >= 0 && tok < p.rows.V ? static_cast<float>((static_cast<double>(x_tok) - sum.m) * p.inv_temperature - log_s)
                                                 : __int_as_float(0x7fffffff);
             p.logprobs[r] = lp;
         }
@@ -1020,7 +1021,7 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
                 const unsigned long long b = sel.best[tid];
                 p.top_ids[r * p.k + tid] = index_of(b);
                 p.top_logprobs[r * p.k + tid] = static_cast<float>(
-                    static_cast<double>(value_of(static_cast<uint32_t>(b >> 32)) - sum.m) * p.inv_temperature - row_log_s);
+                    (static_cast<double>(value_of(static_cast<uint32_t>(b >> 32))) - sum.m) * p.inv_temperature - row_log_s);
             }
         }
     }
@@ -1200,9 +1201,9 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_grad_kernel(const _
 
 // ------------------------------------------------------------------ distillation from a teacher's best tokens
 // q: the teacher's listed tokens, and with a tail one bucket for all others, q_r = 1 - sum q.  p: the student, p_r the sum
-// over the tokens that are not listed.  KL(q || p) (METHOD 0) or KL(p || q) (METHOD 1) over the buckets.  p_r is summed as
+// over the tokens that are not listed.  KL(q || p), or with forward_kl KL(p || q), over the buckets.  p_r is summed as
 // such and not as 1 - sum p, which would leave nothing of a small rest: the listed tokens are bits of a map in shared memory,
-// a byte per vector, and the stream leaves them out.
+// a word for a lane's vectors of a step, and the stream writes minus infinity over them before it reads a stage.
 constexpr double NO_TAIL = 9.5367431640625e-07;     // 2^-20: what 1 - sum q can be by the rounding of fp32 log probabilities
 
 struct DistillArgs {
@@ -1217,15 +1218,16 @@ struct DistillArgs {
     int* entries;                   // [rows][k]: the ids that count, -1 elsewhere
     float* stats;                   // [rows][8]
 };
-// stats: the base m of the gradient's exponentials, 1 / S, factor of p_j at tokens that are not listed, sum q + q_r (METHOD 0) or the loss (METHOD 1), what is taken
-// from the teacher's values to make them log probabilities, 1 / S at temperature one, log S, 1 if the row has any loss
+// stats: the base m of the gradient's exponentials, 1 / S, the factor of p_j at tokens that are not listed, sum q + q_r (with
+// forward_kl the divergence), what is taken from the teacher's values to make them log probabilities, 1 / S at temperature
+// one, log S, 1 if the row has any loss
 
 struct DistillPart {        // of a CTA, relative to its largest logit m
     float m;
     int n;                  // listed tokens that count
     double rest, top, all1; // sums of exponentials: not listed, listed, all at temperature one
-    double q, qx;           // METHOD 0: sum of the teacher's weights u, sum of u (its log - x / temperature)
-    double px;              // METHOD 1: sum of listed exponentials times (x / temperature - teacher's log)
+    double q, qx;           // sum of the teacher's weights u, sum of u (its log - x / temperature)
+    double px;              // forward_kl: sum of listed exponentials times (x / temperature - teacher's log)
 };
 
 // Four CTAs per SM: there is more to do around a row's stream than above, which the others hide (2047 x 50257 bf16: 48 us, 53
@@ -1233,7 +1235,7 @@ struct DistillPart {        // of a CTA, relative to its largest logit m
 template <typename T, AtOne ONE>
 __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
     constexpr int N = Elem<T>::N;
-    extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then a byte per vector of this CTA
+    extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then the map
     uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + ring_bytes(p.stages));
     __shared__ float red[4 * WARPS];
     __shared__ int id_of[MAX_K];
@@ -1475,8 +1477,8 @@ struct DistillGradArgs {
     const float *d_kl, *d_nll;      // either may be null
 };
 
-// Tokens that are not listed: p_j times the row's factor.  Listed ones: p_i (sum q + q_r) - q_i (METHOD 0),
-// p_i (log p_i - log q_i - KL) (METHOD 1).  Both over the temperature, and the cross entropy's p_j - 1[label = j] on top.
+// Tokens that are not listed: p_j times the row's factor.  Listed ones: p_i (sum q + q_r) - q_i, with forward_kl
+// p_i (log p_i - log q_i - KL).  Both over the temperature, and the cross entropy's p_j - 1[label = j] on top.
 template <typename T, AtOne ONE>
 __global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(const __grid_constant__ DistillGradArgs p) {
     const int tid = threadIdx.x;

@@ -7,6 +7,7 @@ no counterpart; its losses go through ``F.log_softmax``, lm_engine/model_wrapper
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -48,7 +49,7 @@ def logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """``(x, inner, ld_inner, ld_outer)``: row ``r`` of ``x`` read as ``[rows, V]`` starts at
     ``(r // inner) * ld_outer + (r % inner) * ld_inner`` elements.  Copied only where no two strides say where its rows
     are, or the vocabulary is not dense."""
-    V = x.size(-1)
+    V = x.shape[-1]
     if x.is_contiguous():
         return x, x.numel() // V or 1, V, 0
     levels: list[tuple[int, int]] = []          # (size, stride) from the inside, dimensions of size 1 left out
@@ -69,15 +70,15 @@ def logit_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
 
 def kernel_usable(logits: torch.Tensor, temperature, *others: torch.Tensor | None) -> bool:
     """A temperature that is a tensor may want a gradient: it is left to the PyTorch operations."""
-    if logits.dtype not in KERNEL_TYPES or isinstance(temperature, torch.Tensor) or logits.size(-1) > 1 << 30:
+    if logits.dtype not in KERNEL_TYPES or isinstance(temperature, torch.Tensor) or logits.shape[-1] > 1 << 30:
         return False
     return _lib.eager(logits, *others)
 
 
 def check_logits(logits: torch.Tensor, temperature) -> None:
-    if logits.dim() == 0 or logits.size(-1) == 0 or (logits.dtype not in KERNEL_TYPES and not logits.is_floating_point()):
+    if not logits.shape or not logits.shape[-1] or (logits.dtype not in KERNEL_TYPES and not logits.is_floating_point()):
         raise ValueError(f"logits need a floating type and a vocabulary, got {logits.dtype} of {tuple(logits.shape)}")
-    if not isinstance(temperature, torch.Tensor) and not 0 < temperature < float("inf"):
+    if not isinstance(temperature, torch.Tensor) and not 0 < temperature < math.inf:
         raise ValueError(f"temperature has to be positive, got {temperature}")
 
 
@@ -179,6 +180,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         return token_logprobs_reference(logits, tokens, top_k, temperature, ignore_index)
     if tokens is not None:
         tokens = as_int64(tokens)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, int(top_k), float(temperature), int(ignore_index)))
-    return TokenLogprobs(*_forward(logits, tokens, int(top_k), float(temperature), int(ignore_index), False)[:4])
+    top_k, temperature, ignore_index = int(top_k), float(temperature), int(ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_k, temperature, ignore_index))
+    logprobs, entropy, top, ids, _ = _forward(logits, tokens, top_k, temperature, ignore_index, False)
+    return TokenLogprobs(logprobs, entropy, top, ids)
