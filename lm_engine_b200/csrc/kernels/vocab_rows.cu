@@ -1220,7 +1220,7 @@ struct DistillArgs {
 };
 // stats: the base m of the gradient's exponentials, 1 / S, the factor of p_j at tokens that are not listed, sum q + q_r (with
 // forward_kl the divergence), what is taken from the teacher's values to make them log probabilities, 1 / S at temperature
-// one, log S, 1 if the row has any loss
+// one, log S, 2 if the row has a divergence, 1 if it has a label only, 0 if neither
 
 struct DistillPart {        // of a CTA, relative to its largest logit m
     float m;
@@ -1458,7 +1458,8 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
             const double moved = static_cast<double>(m2) - all.m, log_s2 = log_s - moved * p.inv_temperature;
             float4* st = reinterpret_cast<float4*>(p.stats + 8 * r);
             st[0] = make_float4(m2, static_cast<float>(exp(-log_s2)), static_cast<float>(factor), static_cast<float>(fourth));
-            st[1] = make_float4(static_cast<float>(norm), static_cast<float>(exp(moved - log_s1)), static_cast<float>(log_s2), 1.f);
+            st[1] = make_float4(static_cast<float>(norm), static_cast<float>(exp(moved - log_s1)), static_cast<float>(log_s2),
+                                all.n > 0 ? 2.f : 1.f);
         }
     }
     if (p.splits > 1) cluster_sync();
@@ -1492,7 +1493,7 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(cons
         return;
     }
     const float m = s0.x, inv_s = s0.y, c = p.inv_temperature * LOG2E;
-    const float d_kl = p.d_kl != nullptr ? p.d_kl[r] * p.inv_temperature : 0.f;
+    const float d_kl = p.d_kl != nullptr && s1.w == 2.f ? p.d_kl[r] * p.inv_temperature : 0.f;
     int label = -1;
     float d_nll = 0.f;
     if (p.d_nll != nullptr) {

@@ -662,3 +662,29 @@ def test_fp32_gradients_of_the_forward_divergence_are_fp32(offset):
                                      .kl_divergence.sum(), x64)
         # p (log p - log q - KL): logarithms of at most 2^5, a few roundings of 2^-24 each, of terms that partly cancel
         assert float((got.double() - ref).norm() / ref.norm()) < 2.0 ** -24 * 2 ** 5 * 4
+
+
+@pytest.mark.parametrize("temperature", [0.5, 0.6, 3.0, 50.0])
+def test_labels_beside_other_temperatures(temperature):
+    for dtype in (BF, F32):
+        x = _rows(1, 40, 20003, dtype, 6)
+        x[..., 9000:] += 4.0
+        for method, tail in METHODS:
+            ids, lq = _lists(x, 16, 2, tail, temperature)
+            _distill(x, ids, lq, ids[..., 3], method, tail, temperature)
+
+
+def test_upstream_gradients_of_rows_without_a_part_are_not_used():
+    from lm_engine_b200.ops import token_logprobs, topk_distillation
+
+    x = _rows(1, 4, 700, BF, 1).requires_grad_(True)
+    ids, lq = _lists(x.detach(), 6, 2)
+    ids[0, 0] = ids[0, 1] = -1
+    labels = torch.tensor([[3, -100, -100, 5]], device="cuda")
+    out = topk_distillation(x, ids, lq, labels)
+    nan = math.nan
+    d_kl, d_nll = torch.tensor([[nan, nan, 1.0, 1.0]], device="cuda"), torch.tensor([[1.0, nan, nan, 1.0]], device="cuda")
+    (g,) = torch.autograd.grad([out.kl_divergence, out.nll], [x], [d_kl, d_nll])
+    assert g.isfinite().all() and float(g[0, 1].abs().max()) == 0 and float(g[0, 0].abs().max()) > 0
+    (g,) = torch.autograd.grad([token_logprobs(x, labels).logprobs], [x], [d_nll])
+    assert g.isfinite().all() and float(g[0, 1:3].abs().max()) == 0
