@@ -1216,16 +1216,18 @@ struct DistillArgs {
     int k, splits, stages, forward_kl, tail;
     float *kl, *nll;
     int* entries;                   // [rows][k]: the ids that count, -1 elsewhere
-    float* stats;                   // [rows][8]
+    float* stats;                   // [rows][12]
 };
-// stats: the base m of the gradient's exponentials, 1 / S, the factor of p_j at tokens that are not listed, sum q + q_r (with
-// forward_kl the divergence), what is taken from the teacher's values to make them log probabilities, 1 / S at temperature
-// one, log S, 2 if the row has a divergence, 1 if it has a label only, 0 if neither
+// stats, for the gradient.  Tokens that are not listed: base m_r of their exponentials, what these are multiplied by for the
+// divergence and for the cross entropy, and 2 if the row has a divergence, 1 if it has a label only, 0 if neither.  Listed ones:
+// base m, 1 / S, log S, sum q + q_r (with forward_kl the divergence); what is taken from the teacher's values to make them log
+// probabilities (in two parts), 1 / S at temperature one.  Two bases, since all that is not listed may be less likely than fp32 can say.
 
-struct DistillPart {        // of a CTA, relative to its largest logit m
-    float m;
+struct DistillPart {        // of a CTA
+    float m, mr;            // largest of its bases, and that of the tokens that are not listed
     int n;                  // listed tokens that count
-    double rest, top, all1; // sums of exponentials: not listed, listed, all at temperature one
+    double rest, rest1;     // sums of exponentials relative to mr: not listed, the same at temperature one
+    double top, top1;       // relative to m: listed
     double q, qx;           // sum of the teacher's weights u, sum of u (its log - x / temperature)
     double px;              // forward_kl: sum of listed exponentials times (x / temperature - teacher's log)
 };
@@ -1275,7 +1277,7 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
                 p.kl[r] = 0.f;
                 if (p.nll != nullptr) p.nll[r] = 0.f;
             }
-            if (tid < 8) p.stats[8 * r + tid] = 0.f;
+            if (tid < 12) p.stats[12 * r + tid] = 0.f;
         }
         return;                         // (all CTAs of the cluster alike)
     }
@@ -1372,13 +1374,7 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
             e[q] = 0;
             for (int i = 0; i < MAX_K / 32; ++i) e[q] += part_of[i][q];
         }
-        double rest = sum.s, rest1 = sum.s1;
-        if (sum.m != m) {
-            const double d = fmax(static_cast<double>(sum.m) - m, -1e30);
-            rest *= exp(d * p.inv_temperature);
-            if (ONE) rest1 *= exp(d);
-        }
-        part = DistillPart{m, n, rest, e[0], ONE ? rest1 + e[1] : 0.0, e[2], p.forward_kl ? 0.0 : e[3], p.forward_kl ? e[3] : 0.0};
+        part = DistillPart{m, sum.m, n, sum.s, sum.s1, e[0], e[1], e[2], p.forward_kl ? 0.0 : e[3], p.forward_kl ? e[3] : 0.0};
     }
     __syncwarp();
     if (p.splits > 1) cluster_sync();
@@ -1388,61 +1384,80 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
             const bool there = lane < p.splits;
             const DistillPart* q = &part;
             all.m = there ? ld_peer(&q->m, lane) : -INFINITY;
+            all.mr = there ? ld_peer(&q->mr, lane) : -INFINITY;
             all.n = there ? ld_peer(&q->n, lane) : 0;
             all.rest = there ? ld_peer(&q->rest, lane) : 0;
             all.top = there ? ld_peer(&q->top, lane) : 0;
-            all.all1 = there && ONE ? ld_peer(&q->all1, lane) : 0;
+            all.rest1 = there && ONE ? ld_peer(&q->rest1, lane) : 0;
+            all.top1 = there && ONE ? ld_peer(&q->top1, lane) : 0;
             all.q = there ? ld_peer(&q->q, lane) : 0;
             all.qx = there ? ld_peer(&q->qx, lane) : 0;
             all.px = there ? ld_peer(&q->px, lane) : 0;
-            float largest = all.m;
+            float largest = all.m, largest_r = all.mr;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            for (int o = 16; o > 0; o >>= 1) {
+                largest = max_nan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+                largest_r = max_nan(largest_r, __shfl_xor_sync(0xffffffffu, largest_r, o));
+            }
             if (there && all.m != largest) {
                 const double d = fmax(static_cast<double>(all.m) - largest, -1e30), f = exp(d * p.inv_temperature);
-                all.rest *= f;
                 all.top *= f;
                 all.px *= f;
-                if (ONE) all.all1 *= exp(d);
+                if (ONE) all.top1 *= exp(d);
+            }
+            if (there && all.mr != largest_r) {
+                const double d = fmax(static_cast<double>(all.mr) - largest_r, -1e30);
+                all.rest *= exp(d * p.inv_temperature);
+                if (ONE) all.rest1 *= exp(d);
             }
             all.m = largest;
-            double* v[6] = {&all.rest, &all.top, &all.all1, &all.q, &all.qx, &all.px};
+            all.mr = largest_r;
+            double* v[7] = {&all.rest, &all.top, &all.rest1, &all.top1, &all.q, &all.qx, &all.px};
 #pragma unroll
             for (int o = MAX_SPLITS / 2; o > 0; o >>= 1) {
                 all.n += __shfl_xor_sync(0xffffffffu, all.n, o);
 #pragma unroll
-                for (int i = 0; i < 6; ++i) *v[i] += __shfl_xor_sync(0xffffffffu, *v[i], o);
+                for (int i = 0; i < 7; ++i) *v[i] += __shfl_xor_sync(0xffffffffu, *v[i], o);
             }
         }
-        // the logarithms, a lane for each, then one thread
-        const double S = all.rest + all.top, S1 = ONE ? all.all1 : S;
+        // the logarithms, a lane for each, then one thread.  What is not listed stays in the logarithm: its probability may be
+        // less than a double can say.
+        const double down = all.rest > 0 ? static_cast<double>(all.mr) - all.m : all.rest == 0 ? 0.0 : all.rest;    // (or NaN)
+        const double S = all.top + all.rest * exp(down * p.inv_temperature);
+        const double S1 = ONE ? all.top1 + all.rest1 * exp(down) : S;
         double q_r = p.tail ? 1 - all.q : 0.0;
         if (q_r < NO_TAIL) q_r = 0;
-        const double logs = log(lane == 0 ? S : lane == 1 ? all.rest : lane == 2 ? fmax(q_r, NO_TAIL) : lane == 3 ? all.q : S1);
-        const double log_s = __shfl_sync(0xffffffffu, logs, 0), log_p_r = __shfl_sync(0xffffffffu, logs, 1) - log_s;
+        const double logs = log(lane == 0   ? S
+                                : lane == 1 ? all.rest
+                                : lane == 2 ? fmax(q_r, NO_TAIL)
+                                : lane == 3 ? all.q
+                                : lane == 4 ? S1
+                                            : all.rest1);
+        const double log_s = __shfl_sync(0xffffffffu, logs, 0), log_rest = __shfl_sync(0xffffffffu, logs, 1);
         const double log_q_r = __shfl_sync(0xffffffffu, logs, 2), log_q = __shfl_sync(0xffffffffu, logs, 3);
-        const double log_s1 = __shfl_sync(0xffffffffu, logs, 4);
+        const double log_s1 = __shfl_sync(0xffffffffu, logs, 4), log_rest1 = __shfl_sync(0xffffffffu, logs, 5);
         if (lane == 0) {
-            const double lse = all.m * p.inv_temperature + log_s;
+            const bool others = all.rest != 0;      // (NaN too)
+            const double lse = all.m * p.inv_temperature + log_s, log_p_r = log_rest + down * p.inv_temperature - log_s;
+            const double p_r = others ? exp(log_p_r) : 0.0;
             double kl = 0, factor = 0, fourth = 0, norm = 0;
             if (all.n > 0) {
-                const double p_r = all.rest / S;
                 if (!p.forward_kl) {
                     if (p.tail) {
                         kl = all.qx + all.q * lse;
                         if (q_r > 0) kl += q_r * (log_q_r - log_p_r);
-                        fourth = all.q + q_r;
+                        fourth = all.q + (others ? q_r : 0.0);
                     } else {
                         norm = ref + log_q;
                         kl = all.qx / all.q - log_q + lse;
                         fourth = 1;
                     }
-                    factor = fourth - (p_r > 0 ? q_r / p_r : 0.0);
+                    factor = fourth * p_r - q_r;
                 } else {
-                    const double ratio = p_r > 0 ? log_p_r - log_q_r : 0.0;
+                    const double ratio = others ? log_p_r - log_q_r : 0.0;
                     kl = (all.px - all.top * lse) / S + p_r * ratio;
                     fourth = kl;
-                    factor = ratio - kl;
+                    factor = p_r * (ratio - kl);
                 }
             }
             p.kl[r] = static_cast<float>(kl);
@@ -1450,16 +1465,22 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
                 p.nll[r] = !labelled              ? 0.f
                            : label >= 0 && label < V ? static_cast<float>(log_s1 - (static_cast<double>(x_label) - all.m))
                                                      : __int_as_float(0x7fffffff);
-            // The gradient's exponentials are relative to where the sums are about one (both of them at least one), so that the
-            // logarithms that it subtracts are small.
-            double up = log_s / p.inv_temperature;
-            if (ONE) up = fmin(up, log_s1);
-            const float m2 = static_cast<float>(all.m + up);
+            // The gradient's exponentials are relative to where their sums are about one (at both temperatures at least one), so
+            // that the logarithms that it subtracts are small.
+            double up = log_s / p.inv_temperature, up_r = log_rest / p.inv_temperature;
+            if (ONE) {
+                up = fmin(up, log_s1);
+                up_r = fmin(up_r, log_rest1);
+            }
+            const float m2 = static_cast<float>(all.m + up), mr2 = others ? static_cast<float>(all.mr + up_r) : S > 0 ? 0.f : m2 - m2;
             const double moved = static_cast<double>(m2) - all.m, log_s2 = log_s - moved * p.inv_temperature;
-            float4* st = reinterpret_cast<float4*>(p.stats + 8 * r);
-            st[0] = make_float4(m2, static_cast<float>(exp(-log_s2)), static_cast<float>(factor), static_cast<float>(fourth));
-            st[1] = make_float4(static_cast<float>(norm), static_cast<float>(exp(moved - log_s1)), static_cast<float>(log_s2),
-                                all.n > 0 ? 2.f : 1.f);
+            const double inv_rest = others ? exp((static_cast<double>(mr2) - all.mr) * p.inv_temperature - log_rest) : 0.0;
+            const double of_nll = ONE ? (others ? exp(static_cast<double>(mr2) - all.m - log_s1) : 0.0) : p_r * inv_rest;
+            float4* st = reinterpret_cast<float4*>(p.stats + 12 * r);
+            st[0] = make_float4(mr2, static_cast<float>(factor * inv_rest), static_cast<float>(of_nll), all.n > 0 ? 2.f : 1.f);
+            st[1] = make_float4(m2, static_cast<float>(exp(-log_s2)), static_cast<float>(log_s2), static_cast<float>(fourth));
+            const float norm_hi = static_cast<float>(norm);     // (raw logits may have any offset)
+            st[2] = make_float4(norm_hi, static_cast<float>(norm - norm_hi), static_cast<float>(exp(moved - log_s1)), 0.f);
         }
     }
     if (p.splits > 1) cluster_sync();
@@ -1487,13 +1508,14 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(cons
     const int V = p.rows.V;
     T* out = static_cast<T*>(p.grad) + r * V;
     const GradSlice<T> g(p.rows.row<T>(r), out, V, blockIdx.x % static_cast<unsigned>(p.chunks), p.steps);
-    const float4 s0 = reinterpret_cast<const float4*>(p.stats + 8 * r)[0], s1 = reinterpret_cast<const float4*>(p.stats + 8 * r)[1];
-    if (s1.w == 0.f) {              // no loss: not read, gradient zero
+    const float4* st = reinterpret_cast<const float4*>(p.stats + 12 * r);
+    const float4 others = st[0];
+    if (others.w == 0.f) {          // no loss: not read, gradient zero
         g.zero();
         return;
     }
-    const float m = s0.x, inv_s = s0.y, c = p.inv_temperature * LOG2E;
-    const float d_kl = p.d_kl != nullptr && s1.w == 2.f ? p.d_kl[r] * p.inv_temperature : 0.f;
+    const float c = p.inv_temperature * LOG2E;
+    const float d_kl = p.d_kl != nullptr && others.w == 2.f ? p.d_kl[r] * p.inv_temperature : 0.f;
     int label = -1;
     float d_nll = 0.f;
     if (p.d_nll != nullptr) {
@@ -1503,10 +1525,10 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(cons
             d_nll = p.d_nll[r];
         }
     }
-    const float a = d_kl * inv_s * s0.z + (ONE ? 0.f : d_nll * inv_s), a1 = d_nll * s1.y;
-    const unsigned long long nm = pair(-m, -m), cc = pair(c, c), cc1 = pair(LOG2E, LOG2E), aa = pair(a, a), aa1 = pair(a1, a1);
-    auto t_of = [&](float x) { return (x - m) * c; };
-    auto value = [&](unsigned long long x) {
+    const float a = d_kl * others.y + (ONE ? 0.f : d_nll * others.z), a1 = d_nll * others.z;
+    const unsigned long long nm = pair(-others.x, -others.x), cc = pair(c, c), cc1 = pair(LOG2E, LOG2E), aa = pair(a, a);
+    const unsigned long long aa1 = pair(a1, a1);
+    auto value = [&](unsigned long long x) {        // (at listed tokens it may run over: they get theirs below)
         const unsigned long long d = add2(x, nm);
         const float2 t = halves(mul2(d, cc));
         const unsigned long long e = pair(exp2_approx(t.x), exp2_approx(t.y)), v = mul2(e, aa);
@@ -1521,12 +1543,13 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(cons
     const bool here = g.has(id), met = here && id == label;
     const bool taken = __syncthreads_or(met);
     if (here) {
-        const float x = Elem<T>::f(g.x[id]), t = t_of(x), e = exp2_approx(t) * inv_s;
-        const float lq = p.teacher[r * p.k + tid] - s1.x;
+        const float4 top = st[1], more = st[2];
+        const float d = Elem<T>::f(g.x[id]) - top.x, t = d * c, e = exp2_approx(t) * top.y;
+        const float lq = p.teacher[r * p.k + tid] - more.x - more.y;
         float v;
-        if (p.forward_kl) v = e == 0.f ? 0.f : e * (t * static_cast<float>(LN2) - s1.z - lq - s0.w);
-        else v = e * s0.w - __expf(lq);
-        v = v * d_kl + d_nll * (ONE ? exp2_approx((x - m) * LOG2E) * s1.y : e) - (met ? d_nll : 0.f);
+        if (p.forward_kl) v = e == 0.f ? 0.f : e * (t * static_cast<float>(LN2) - top.z - lq - top.w);
+        else v = e * top.w - __expf(lq);
+        v = v * d_kl + d_nll * (ONE ? exp2_approx(d * LOG2E) * more.z : e) - (met ? d_nll : 0.f);
         out[id] = Elem<T>::from(v);
     }
     if (tid == 0 && !taken && g.has(label)) {

@@ -396,7 +396,7 @@ int lme_token_logprobs_bwd(const void* x, int dtype, long long rows, long long i
 // probability is 1 - the listed ones' (needed by forward_kl); without it the teacher's values are renormalised.  Entries with an id
 // outside of [0, V) or a value of -inf are absent, an id's later entries too; a row without entries has kl 0.  labels / nll
 // (both or neither): cross entropy at temperature one, 0 where a label is ignore_index.  entries (int [rows, k]) and stats
-// (8 floats per row, 16-byte aligned) are what the gradient needs.
+// (12 floats per row, 16-byte aligned) are what the gradient needs.
 int lme_topk_distillation_fwd(const void* x, int dtype, long long rows, long long inner, long long ld_inner,
                               long long ld_outer, int V, const long long* top_ids, const float* top_logprobs, int k,
                               const long long* labels, long long ignore_index, double temperature, int forward_kl, int tail,

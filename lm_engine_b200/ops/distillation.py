@@ -49,26 +49,28 @@ def topk_distillation_reference(logits: torch.Tensor, top_ids: torch.Tensor, top
     x = torch.where(read[..., None], x, 0.0)                    # other rows are not looked at
     logp = torch.log_softmax(x / temperature, -1)
     listed = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add_(-1, ids, there.int()) > 0
-    p_rest = torch.where(listed, 0.0, logp.exp()).sum(-1).double()
+    others = logp.double().masked_fill(listed, -torch.inf)      # in the logarithm: they may be less likely than a number can say
+    none = (others == -torch.inf).all(-1)
+    log_rest = torch.where(none, -torch.inf, others.masked_fill(none[..., None], 0.0).logsumexp(-1))
     student = torch.where(there, logp.gather(-1, ids).double(), 0.0)
     teacher = torch.where(there, teacher, -torch.inf)
     if not tail:
         teacher = teacher - torch.where(asked, teacher.logsumexp(-1), 0.0)[..., None]
     q = teacher.exp()
-    q_rest = torch.zeros_like(p_rest)
+    q_rest = torch.zeros_like(log_rest)
     if tail:
         q_rest = 1 - q.sum(-1)
         q_rest = torch.where(q_rest < NO_TAIL, 0.0, q_rest)
-    log_rest = torch.where(p_rest > 0, p_rest, 1.0).log()
     if kl_divergence_method == KLDivergenceMethod.backward:
         kl = torch.where(q > 0, q * (teacher - student), 0.0).sum(-1)
-        rest = q_rest * (q_rest.clamp(min=NO_TAIL).log() - torch.where(p_rest > 0, log_rest, -torch.inf))
+        rest = q_rest * (q_rest.clamp(min=NO_TAIL).log() - log_rest)
         kl = kl + torch.where(q_rest > 0, rest, 0.0)
     else:
         finite = there & (student != -torch.inf)
         away = torch.where(finite, student, 0.0) - torch.where(finite, teacher, 0.0)
         kl = torch.where(finite, student.exp() * away, 0.0).sum(-1)
-        kl = kl + torch.where(p_rest > 0, p_rest * (log_rest - q_rest.clamp(min=NO_TAIL).log()), 0.0)
+        log_rest = torch.where(none, 0.0, log_rest)
+        kl = kl + torch.where(none, 0.0, log_rest.exp() * (log_rest - q_rest.clamp(min=NO_TAIL).log()))
     kl = torch.where(asked, kl, 0.0).to(x.dtype)
     if labels is None:
         return TopkDistillation(kl, None)
@@ -91,7 +93,7 @@ class _TopkDistillation(torch.autograd.Function):
             kl = torch.empty_like(labels, dtype=torch.float32)
             nll = torch.empty_like(kl)
         ctx.entries = torch.empty_like(top_ids, dtype=torch.int32)
-        ctx.stats = torch.empty(8 * rows, dtype=torch.float32, device=x.device)
+        ctx.stats = torch.empty(12 * rows, dtype=torch.float32, device=x.device)
         rc = _lib.cuda_lib().lme_topk_distillation_fwd(
             x.data_ptr(), KERNEL_TYPES[x.dtype], rows, inner, ld_inner, ld_outer, V, top_ids.data_ptr(),
             top_logprobs.data_ptr(), K, _lib.ptr(labels), ignore_index, temperature,

@@ -73,9 +73,17 @@ def _score(x, tok, k, temperature, seed=0, grads=True):
     size = sum((d.abs().sum(-1) if d.dim() > p.dim() - 1 else d.abs())[..., None] for _, _, d in pairs)
     size = (size * (2 + logp.clamp(min=-300).abs() + math.log2(V + 1)) / temperature).nan_to_num(0)     # terms that add up to
     eps = torch.finfo(x.dtype).eps / 2                                                                # a gradient, over p
-    # an exponential below 2^-126 counts as none: off by that times the same factors (the sum that divides it is one at least)
-    tiny = size * 2.0 ** -126 + (2.0 ** -25 if x.dtype == HF else 2.0 ** -126)
-    _check(got, ref, ref.abs().nan_to_num(0) * (eps + 2.0 ** -22) + (p * size).nan_to_num(0) * (4 * e) + tiny, "gradient")
+    patch = torch.zeros_like(p)                     # upstream values of single tokens, scaled and added in fp32
+    if tok is not None:
+        here = (tok >= 0) & (tok < V)
+        patch.scatter_add_(-1, torch.where(here, tok, 0).long()[..., None], torch.where(here, pairs[0][2].abs(), 0.0).double()[..., None])
+    if k:
+        patch.scatter_add_(-1, out.top_ids, pairs[-1][2].abs().double())
+    size_p = (p * size).nan_to_num(0) * (4 * e) + patch / temperature * 2.0 ** -22
+    # an exponential below 2^-126 counts as none: off by that times the same factors, over a sum of 2^-1/2 at least (a thread's
+    # base is its sum's logarithm rounded to a power of two)
+    tiny = size * 2.0 ** -125.5 + (2.0 ** -25 if x.dtype == HF else 2.0 ** -126)
+    _check(got, ref, ref.abs().nan_to_num(0) * (eps + 2.0 ** -22) + size_p + tiny, "gradient")
     return out
 
 
@@ -220,10 +228,11 @@ def _distill(x, ids, lq, labels, method, tail, temperature, seed=0, slack=1.0):
     q = torch.zeros_like(p).scatter_add_(-1, torch.where(inside, ids, 0), torch.where(inside, lq.double(), -math.inf).exp())
     if not tail:
         q = q / q.sum(-1, keepdim=True).clamp(min=1e-30)
-    rest = torch.where(q > 0, 0.0, p).sum(-1, keepdim=True)
-    over = ((1 - q.sum(-1, keepdim=True)).clamp(min=0) / rest.clamp(min=1e-300)) if tail else torch.zeros_like(rest)
+    # the teacher's rest is spread over what is not listed as the student has it
+    rest = (1 - q.sum(-1, keepdim=True)).clamp(min=0) if tail else torch.zeros_like(kl)[..., None]
+    share = torch.softmax((x64.detach() / temperature).masked_fill(q > 0, -math.inf), -1).nan_to_num(0)
     if method == "backward":
-        terms = p * (1 + over) + q
+        terms = p + q + rest * share
     else:
         terms = p * (4 + p.clamp(min=1e-30).log().abs() + q.clamp(min=2.0 ** -20).log().abs() + math.log2(V + 2)
                      + kl.abs()[..., None] + torch.where(q > 0, lq.double().abs().clamp(max=1e4).amax(-1, keepdim=True), 0.0))
@@ -232,7 +241,7 @@ def _distill(x, ids, lq, labels, method, tail, temperature, seed=0, slack=1.0):
         terms = terms + torch.softmax(x64.detach(), -1) * d[1].abs()[..., None]
     eps = torch.finfo(x.dtype).eps / 2
     # an exponential below 2^-126 counts as none: off by that times what terms has beside p
-    flushed = (1 + over) if method == "backward" else 4 + 300 + kl.abs()[..., None] + lq.double().abs().clamp(max=1e4).amax(-1, keepdim=True)
+    flushed = 2.0 if method == "backward" else 4 + 300 + kl.abs()[..., None] + lq.double().abs().clamp(max=1e4).amax(-1, keepdim=True)
     tiny = 2.0 ** -126 * (flushed * d[0].abs()[..., None] / temperature + 1).nan_to_num(0, 0, 0)
     tiny = tiny + (2.0 ** -25 if x.dtype == HF else 2.0 ** -126)
     _check(got, ref, ref.abs().nan_to_num(0) * (eps + 2.0 ** -22) + terms.nan_to_num(0) * (4 * e * slack) + tiny, "gradient")
@@ -688,3 +697,24 @@ def test_upstream_gradients_of_rows_without_a_part_are_not_used():
     assert g.isfinite().all() and float(g[0, 1].abs().max()) == 0 and float(g[0, 0].abs().max()) > 0
     (g,) = torch.autograd.grad([token_logprobs(x, labels).logprobs], [x], [d_nll])
     assert g.isfinite().all() and float(g[0, 1:3].abs().max()) == 0
+
+
+@pytest.mark.parametrize("gap", [60.0, 100.0, 300.0, 2000.0])
+@pytest.mark.parametrize("method,tail", METHODS)
+def test_lists_that_hold_all_but_nothing(gap, method, tail):
+    """What is not listed is less likely than fp32 or fp64 can say; its gradient is the teacher's rest all the same."""
+    V = 5003
+    for dtype, temperature in ((F32, 1.0), (BF, 2.0), (F32, 0.7)):
+        x = _rows(1, 12, V, dtype, 4) - gap
+        ids, lq = _lists(x, 10, 3, tail, temperature)
+        x = x.scatter(-1, ids, x.gather(-1, ids) + gap)
+        lq = lq - 0.05 if tail else lq
+        _distill(x, ids, lq, ids[..., 1], method, tail, temperature)
+    x = _rows(1, 3, V, F32, 4)
+    x[0, 1] = -math.inf
+    from lm_engine_b200.ops import topk_distillation
+
+    leaf = x.requires_grad_(True)
+    out = topk_distillation(leaf, ids[:, :3], lq[:, :3], None, method, tail)
+    (g,) = torch.autograd.grad(out.kl_divergence.sum(), leaf)
+    assert out.kl_divergence[0, 1].isnan() and g[0, 1].isnan().all() and g[0, 0].isfinite().all()
