@@ -11,9 +11,10 @@
 // instructions per logit take: a CTA of 256 threads streams a row through rings of bulk copies, one per warp; rows are split
 // over a cluster of up to 8 CTAs when there are few of them, and joined through distributed shared memory: one launch, no
 // workspace, a fixed order of sums.
-// Measured on a B200 (1000 W, sustained): scores of 4094 x 128256 bf16 logits 171 us = 6.1 TB/s, with the best 64 of 4096
-// rows 220 us = 4.8 TB/s (selection: 12 of the 42 thousand cycles of a row); gradient at 4096 x 128256 327 us = 6.4 TB/s;
-// distillation at 8192 x 128256 with the best 64, forward 348 us = 6.0 TB/s, backward 648 us = 6.5 TB/s.
+// Measured on a B200 (1000 W, sustained; up to 12 % more on others, at lower clocks): scores of 4094 x 128256 bf16
+// logits 171 us = 6.1 TB/s, with the best 64 of 4096 rows 220 us = 4.8 TB/s (selection: 12 of the 42 thousand cycles of
+// a row); gradient at 4096 x 128256 327 us = 6.4 TB/s; distillation at 8192 x 128256 with the best 64, forward 348 us =
+// 6.0 TB/s, backward 648 us = 6.5 TB/s.
 // Included by lme_cuda.cu after decode_attention.cu.
 #include <cuda_fp16.h>
 
