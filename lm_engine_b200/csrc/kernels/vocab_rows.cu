@@ -76,7 +76,6 @@ struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
     static constexpr int N = 8;         // per vector
-    static constexpr int KEY_BITS = 16; // of an ordered key that differ between values
     static constexpr uint32_t NEG_INF = 0xff80ff80u;
     static constexpr uint32_t LOW2 = 0xf14af14au;       // two of LOW
     static constexpr float LOW = -1.00025555e30f;
@@ -106,7 +105,6 @@ struct Elem<__nv_bfloat16> {
 template <>
 struct Elem<__half> {
     static constexpr int N = 8;
-    static constexpr int KEY_BITS = 19; // fp16 as fp32 bits: 13 zeros at the end
     static constexpr uint32_t NEG_INF = 0xfc00fc00u;
     static constexpr uint32_t LOW2 = 0xfbfffbffu;
     static constexpr float LOW = -65504.f;
@@ -142,7 +140,6 @@ struct Elem<__half> {
 template <>
 struct Elem<float> {
     static constexpr int N = 4;
-    static constexpr int KEY_BITS = 20; // the selection's first bound may be coarse
     static constexpr uint32_t NEG_INF = 0xff800000u;
     static constexpr uint32_t LOW2 = 0;
     static constexpr float LOW = 0.f;                   // (one value per word: nothing is gained)
@@ -1585,6 +1582,7 @@ inline cudaError_t launch(Kern kern, const Args& a, long long ctas, int splits, 
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+inline bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 inline int elem_size(int dtype) { return dtype == LME_F32 ? 4 : 2; }
 // Steps of a gradient's CTA: eight where that still makes many CTAs, so that what it has to know of its row costs little, else
 // four, fewer where SMs would be idle.  Distillation at 8192 x 128256 bf16, backward: 656 us with eight, 668 with four, 741
@@ -1631,6 +1629,10 @@ extern "C" int lme_token_logprobs_fwd(const void* x, int dtype, long long rows, 
     if (V > MAX_V || rows > MAX_GRID) return LME_ERR_TOO_LARGE;
     const int splits = splits_for(rows, V, elem_size(dtype));
     if (rows * splits > MAX_GRID) return LME_ERR_TOO_LARGE;
+    if (x == nullptr || entropy == nullptr || (tokens != nullptr && logprobs == nullptr) ||
+        (k > 0 && (top_logprobs == nullptr || top_ids == nullptr)))
+        return LME_ERR_SHAPE;
+    if (misaligned(stats)) return LME_ERR_ALIGN;
     const ScoreArgs a{{x, inner, ld_inner, ld_outer, V}, tokens, ignore_index, 1.0 / temperature, k, splits, RING_STAGES, logprobs, entropy,
                       top_logprobs, top_ids, stats};
     const long long ctas = rows * splits;
@@ -1653,6 +1655,8 @@ extern "C" int lme_token_logprobs_bwd(const void* x, int dtype, long long rows, 
     if (V > MAX_V) return LME_ERR_TOO_LARGE;
     const GradGrid grid = grad_grid(rows, V, elem_size(dtype));
     if (rows * grid.chunks > MAX_GRID) return LME_ERR_TOO_LARGE;
+    if (x == nullptr || grad == nullptr || stats == nullptr || (d_top != nullptr && top_ids == nullptr)) return LME_ERR_SHAPE;
+    if (misaligned(stats)) return LME_ERR_ALIGN;
     const ScoreGradArgs a{{x, inner, ld_inner, ld_outer, V}, grad, tokens, ignore_index, static_cast<float>(1.0 / temperature), k,
                           grid.chunks, grid.steps, stats, top_ids, d_logprobs, d_entropy, d_top};
     const long long ctas = rows * grid.chunks;
@@ -1700,6 +1704,9 @@ extern "C" int lme_topk_distillation_fwd(const void* x, int dtype, long long row
     auto map_bytes = [&](int s) { return ((((V + 2 * n - 2) / n + s - 1) / s + WARP_STEP - 1) / WARP_STEP * 32 + 4) * 4; };
     while (splits < MAX_SPLITS && map_bytes(splits) > MAX_MAP) splits *= 2;
     if (map_bytes(splits) > MAX_MAP || rows * splits > MAX_GRID) return LME_ERR_TOO_LARGE;
+    if (x == nullptr || top_ids == nullptr || top_logprobs == nullptr || kl == nullptr || entries == nullptr || stats == nullptr)
+        return LME_ERR_SHAPE;
+    if (misaligned(stats)) return LME_ERR_ALIGN;
     const DistillArgs a{{x, inner, ld_inner, ld_outer, V}, top_ids, top_logprobs, labels, ignore_index, 1.0 / temperature, k,
                         splits, RING_STAGES, forward_kl, tail, kl, nll, entries, stats};
     const AtOne one = at_one(labels != nullptr, temperature);
@@ -1723,6 +1730,8 @@ extern "C" int lme_topk_distillation_bwd(const void* x, int dtype, long long row
     if (V > MAX_V) return LME_ERR_TOO_LARGE;
     const GradGrid grid = grad_grid(rows, V, elem_size(dtype));
     if (rows * grid.chunks > MAX_GRID) return LME_ERR_TOO_LARGE;
+    if (x == nullptr || grad == nullptr || stats == nullptr || entries == nullptr || top_logprobs == nullptr) return LME_ERR_SHAPE;
+    if (misaligned(stats)) return LME_ERR_ALIGN;
     const DistillGradArgs a{{x, inner, ld_inner, ld_outer, V}, grad, entries, top_logprobs, labels, ignore_index,
                             static_cast<float>(1.0 / temperature), k, grid.chunks, grid.steps, forward_kl, stats, d_kl, d_nll};
     const AtOne one = at_one(d_nll != nullptr, temperature);

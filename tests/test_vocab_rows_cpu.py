@@ -200,6 +200,12 @@ def test_entry_points_refuse_on_the_host():
                                       None) == -6
     assert lib.lme_token_logprobs_fwd(None, 0, 1 << 31, 1, 8, 8, 8, None, -100, 1.0, 0, None, None, None, None, None,
                                       None) == -6
+    # nothing to write to, and statistics that are not on 16 bytes
+    assert lib.lme_token_logprobs_fwd(None, 0, 1, 1, 8, 8, 8, None, -100, 1.0, 0, None, None, None, None, None, None) == -1
+    assert lib.lme_token_logprobs_fwd(16, 0, 1, 1, 8, 8, 8, None, -100, 1.0, 2, None, 16, None, 16, None, None) == -1
+    assert lib.lme_token_logprobs_fwd(16, 0, 1, 1, 8, 8, 8, None, -100, 1.0, 0, None, 16, None, None, 8, None) == -2
+    assert lib.lme_token_logprobs_bwd(16, 0, 1, 1, 8, 8, 8, None, -100, 1.0, 0, None, None, None, None, None, 16, None) == -1
+    assert lib.lme_topk_distillation_bwd(16, 0, 1, 1, 8, 8, 8, None, 16, 2, None, -100, 1.0, 0, 16, None, None, 16, None) == -1
     assert lib.lme_token_logprobs_fwd(None, 0, 0, 1, 8, 8, 8, None, -100, 1.0, 0, None, None, None, None, None, None) == 0
 
 
