@@ -8,26 +8,26 @@
 // per row are finished too.
 //
 // Bound by HBM (one read of the logits forward, a read and a write backward) and, sustained, by the power that the
-// instructions per logit take: a CTA of 256 threads streams a row through rings of bulk copies, one per warp; rows are split
+// instructions per logit take: a CTA of 128 threads streams a row through rings of bulk copies, one per warp; rows are split
 // over a cluster of up to 8 CTAs when there are few of them, and joined through distributed shared memory: one launch, no
 // workspace, a fixed order of sums.
-// Measured on a B200 (1000 W, sustained; up to 12 % more on others, at lower clocks): scores of 4094 x 128256 bf16
-// logits 171 us = 6.1 TB/s, with the best 64 of 4096 rows 220 us = 4.8 TB/s (selection: 12 of the 42 thousand cycles of
-// a row); gradient at 4096 x 128256 327 us = 6.4 TB/s; distillation at 8192 x 128256 with the best 64, forward 348 us =
-// 6.0 TB/s, backward 648 us = 6.5 TB/s.
+// Measured on a B200 (1000 W, sustained; up to 12 % more or less on others): scores of 4094 x 128256 bf16 logits 182 us
+// = 5.8 TB/s, with the best 64 of 4096 rows 237 us = 4.4 TB/s; gradient at 4096 x 128256 328 us = 6.4 TB/s;
+// distillation at 8192 x 128256 with the best 64, forward 344 us = 6.1 TB/s, backward 644 us = 6.5 TB/s.
 // Included by lme_cuda.cu after decode_attention.cu.
 #include <cuda_fp16.h>
 
 namespace lme {
 namespace vr {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
 constexpr int WARPS = THREADS / 32;
 constexpr int UNROLL = 4;               // vectors of 16 bytes per thread and step
 constexpr int WARP_STEP = 32 * UNROLL;  // vectors of a warp and step
+constexpr int RING_STAGES = 2;
 constexpr int MAX_SPLITS = 8;           // CTAs of a cluster
 constexpr int MAX_K = LME_VOCAB_MAX_K;  // best tokens, or tokens of a teacher, per row
-constexpr int SEGMENTS = 8;             // of a CTA's steps: what the selection reads again goes by their maxima
+constexpr int SEGMENTS = 16;            // of a CTA's steps: what the selection reads again goes by their maxima
 constexpr int MAX_CANDIDATES = 1024;
 constexpr int MAX_MAP = 96 * 1024;      // bytes of the map of listed tokens, a byte for each vector of a CTA
 constexpr float T_MIN = -150.f;         // 2^-150 is zero here; keeps 0 * (-inf) out of the sums
@@ -160,6 +160,18 @@ struct Elem<float> {
     static __device__ __forceinline__ float from(float x) { return x; }
 };
 
+// element i of a vector, in registers or shared memory (by bytes: the two types may not alias)
+template <typename T>
+__device__ __forceinline__ void put(uint4& v, int i, T x) {
+    memcpy(reinterpret_cast<unsigned char*>(&v) + i * sizeof(T), &x, sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ T get(const uint4& v, int i) {
+    T x;
+    memcpy(&x, reinterpret_cast<const unsigned char*>(&v) + i * sizeof(T), sizeof(T));
+    return x;
+}
+
 // ------------------------------------------------------------------ rows and their slices
 // Row r starts at x + (r / inner) * ld_outer + (r % inner) * ld_inner: sequences whose last positions are left out are
 // read in place.
@@ -221,11 +233,10 @@ struct Slice {
     // a part, minus infinity where the row is not
     __device__ __forceinline__ uint4 load_part(int j) const {
         uint4 r = nothing();
-        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int v = index(j, i);
-            if (v >= 0 && v < V) e[i] = row[v];
+            if (v >= 0 && v < V) put(r, i, row[v]);
         }
         return r;
     }
@@ -243,17 +254,19 @@ struct Slice {
 template <typename T>
 struct Ring {
     static constexpr uint32_t BYTES = WARP_STEP * 16;
-    uint32_t buf, full;     // shared addresses of this warp's stages and barriers
+    // shared addresses of this warp's stages and barriers; these have memory of their own: written over by ordinary stores, even once
+    // they had been used for the last time, they came back over what was stored
+    uint32_t buf, full;
     const T* source;        // of the next request
     int stages, steps;      // steps: those in which this warp has vectors
     int last;               // vectors of the last one
     int ahead;              // requests so far
     bool ok;
 
-    __device__ __forceinline__ Ring(const Slice<T>& sl, uint8_t* smem, int stages_) : stages(stages_), ahead(0), ok(true) {
+    __device__ __forceinline__ Ring(const Slice<T>& sl, uint8_t* smem, uint64_t* barriers, int stages_) : stages(stages_), ahead(0), ok(true) {
         const int warp = threadIdx.x >> 5;
         buf = smem_u32(smem) + warp * stages * BYTES;
-        uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * stages * BYTES) + warp * stages;
+        uint64_t* bars = barriers + warp * stages;
         full = smem_u32(bars);
         const int j = sl.full0 + warp * WARP_STEP;
         steps = j < sl.full1 ? (sl.full1 - j - 1) / (THREADS * UNROLL) + 1 : 0;
@@ -344,7 +357,7 @@ __device__ __forceinline__ float max_of(const uint4 (&r)[U]) {
     return Elem<T>::max_halves(w);
 }
 
-__host__ __device__ constexpr int ring_bytes(int stages) { return WARPS * stages * (WARP_STEP * 16 + 8); }
+__host__ __device__ constexpr int ring_bytes(int stages) { return WARPS * stages * WARP_STEP * 16; }
 
 // ------------------------------------------------------------------ running sums of a thread
 // m: a base that no logit so far is above by more than SLACK / c, s: sum of 2^t, w: sum of 2^t t with t = (x - m) c.  The base
@@ -583,7 +596,7 @@ __device__ __forceinline__ unsigned long long candidate(uint32_t key, int index)
 }
 __device__ __forceinline__ int index_of(unsigned long long c) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(c)); }
 
-constexpr int BINS = 256;
+constexpr int BINS = 256;               // eight bits of a key
 struct Selection {
     unsigned long long cand[MAX_CANDIDATES];
     unsigned long long best[MAX_K];
@@ -763,8 +776,7 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
         sel.hi[warp] = hi;
         sel.lo[warp] = lo;
     }
-    static_assert(BINS == THREADS, "");
-    sel.bin[tid] = 0;
+    for (int i = tid; i < BINS; i += THREADS) sel.bin[i] = 0;
     __syncthreads();
     uint32_t top = 0, bottom = 0xffffffffu;
 #pragma unroll
@@ -791,7 +803,7 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
         uint32_t prefix = 0;
         int need = k;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            sel.bin[tid] = 0;
+            for (int i = tid; i < BINS; i += THREADS) sel.bin[i] = 0;
             __syncthreads();
             if (some && (shift == 24 || key >> (shift + 8) == prefix)) atomicAdd(&sel.bin[key >> shift & 255], 1);
             __syncthreads();
@@ -862,7 +874,7 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
             for (; hits != 0; hits &= hits - 1) {
                 const int b = __ffs(hits) - 1, a = b / N;
                 const int id = sl.index(a == 0 ? at[0] : a == 1 ? at[1] : a == 2 ? at[2] : at[3], b % N);
-                const float x = Elem<T>::f(reinterpret_cast<const T*>(&sel.stash[a][tid])[b % N]);
+                const float x = Elem<T>::f(get<T>(sel.stash[a][tid], b % N));
                 // (0 for the places of a part that are not the row's: they come last)
                 if (to < MAX_CANDIDATES) sel.cand[to] = id >= 0 && id < sl.V ? candidate(key_of(x), id) : 0ull;
                 ++to;
@@ -888,11 +900,13 @@ struct ScoreArgs {
     float* stats;                   // [rows][4]: m, S, entropy, log S; or null
 };
 
-// Three CTAs per SM with 80 registers: with four and 64 the tried steps take 13 % more instructions (4094 x 128256 bf16,
-// sustained: 186 and 191 us; with the best 64: 233 and 249).
+// Six CTAs of four warps per SM with 80 registers: with more and fewer registers the tried steps take more instructions
+// (4094 x 128256 bf16, sustained: 183 us, 189 with seven; three CTAs of eight warps: 190, and 52 instead of 27 at 8192 x 2048,
+// where what surrounds a row's stream counts).
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid_constant__ ScoreArgs p) {
+__global__ void __launch_bounds__(THREADS, 6) token_logprobs_kernel(const __grid_constant__ ScoreArgs p) {
     __shared__ float red[4 * WARPS];
+    __shared__ uint64_t ring_bars[WARPS * RING_STAGES];
     __shared__ float part_m;
     __shared__ double part_s, part_w, row_log_s;
     __shared__ int part_n;
@@ -908,7 +922,7 @@ __global__ void __launch_bounds__(THREADS, 3) token_logprobs_kernel(const __grid
     const Slice<T> sl(row, p.rows.V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
 
-    Ring<T> ring(sl, vocab_smem, p.stages);
+    Ring<T> ring(sl, vocab_smem, ring_bars, p.stages);
     long long tok = 0;              // of the thread that finishes the row
     float x_tok = 0.f;
     if (p.tokens != nullptr && rank == 0 && tid == THREADS - 1) {
@@ -1072,11 +1086,10 @@ struct GradSlice {
                     v[u] = *reinterpret_cast<const uint4*>(at(x, q));
                     continue;
                 }
-                T* e = reinterpret_cast<T*>(&v[u]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int k = q * N + i - before;
-                    e[i] = k >= 0 && k < V ? x[k] : Elem<T>::from(0.f);
+                    put(v[u], i, k >= 0 && k < V ? x[k] : Elem<T>::from(0.f));
                 }
             }
         }
@@ -1095,11 +1108,10 @@ struct GradSlice {
                     *reinterpret_cast<uint4*>(const_cast<T*>(at(out, q))) = v[u];
                     continue;
                 }
-                const T* e = reinterpret_cast<const T*>(&v[u]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int k = q * N + i - before;
-                    if (k >= 0 && k < V) out[k] = e[i];
+                    if (k >= 0 && k < V) out[k] = get<T>(v[u], i);
                 }
             }
         }
@@ -1148,7 +1160,7 @@ struct ScoreGradArgs {
 
 // dx_j = (1 / temperature) (d_tok (1[tok = j] - p_j) - d_ent p_j (log p_j + H) + sum_i d_top_i (1[id_i = j] - p_j))
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 4) token_logprobs_grad_kernel(const __grid_constant__ ScoreGradArgs p) {
+__global__ void __launch_bounds__(THREADS, 8) token_logprobs_grad_kernel(const __grid_constant__ ScoreGradArgs p) {
     __shared__ float red[32];
     const int tid = threadIdx.x;
     const long long r = blockIdx.x / static_cast<unsigned>(p.chunks);
@@ -1230,14 +1242,14 @@ struct DistillPart {        // of a CTA
     double px;              // forward_kl: sum of listed exponentials times (x / temperature - teacher's log)
 };
 
-// Four CTAs per SM: there is more to do around a row's stream than above, which the others hide (2047 x 50257 bf16: 48 us, 53
-// with three and more registers; 8192 x 128256: 366 and 364).
+// As above (8192 x 128256 bf16: 350 us, 375 with eight CTAs of fewer registers; 2047 x 50257: 46 and 44).
 template <typename T, AtOne ONE>
-__global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
+__global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
     constexpr int N = Elem<T>::N;
     extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then the map
     uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + ring_bytes(p.stages));
     __shared__ float red[4 * WARPS];
+    __shared__ uint64_t ring_bars[WARPS * RING_STAGES];
     __shared__ int id_of[MAX_K];
     __shared__ DistillPart part;
     __shared__ double part_of[MAX_K / 32][4];
@@ -1251,7 +1263,7 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
     const Slice<T> sl(row, V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
 
-    Ring<T> ring(sl, vocab_smem, p.stages);
+    Ring<T> ring(sl, vocab_smem, ring_bars, p.stages);
     // the list: entries that count are in the vocabulary, have a finite or NaN value, and come first of their token
     static_assert(UNROLL == 4, "a word of the map has a lane's vectors of a step");
     const int words = (sl.full1 - sl.full0 + WARP_STEP - 1) / WARP_STEP * 32;       // and one each for the parts at the ends
@@ -1315,10 +1327,9 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_kernel(const __g
         });
     if ((tid == 0 && sl.head) || (tid == 1 && sl.tail)) {
         uint4 v[1] = {sl.load_part(tid == 0 ? 0 : sl.nv - 1)};
-        T* e = reinterpret_cast<T*>(&v[0]);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (listed[words + tid] >> i & 1u) e[i] = Elem<T>::from(-INFINITY);
+            if (listed[words + tid] >> i & 1u) put(v[0], i, Elem<T>::from(-INFINITY));
         run.template add<T>(v, false, [&] { return max_of<T>(v); }, c, LOG2E);
     }
     Sums sum = join_block(run, c, LOG2E, red);
@@ -1500,7 +1511,7 @@ struct DistillGradArgs {
 // Tokens that are not listed: p_j times the row's factor.  Listed ones: p_i (sum q + q_r) - q_i, with forward_kl
 // p_i (log p_i - log q_i - KL).  Both over the temperature, and the cross entropy's p_j - 1[label = j] on top.
 template <typename T, AtOne ONE>
-__global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(const __grid_constant__ DistillGradArgs p) {
+__global__ void __launch_bounds__(THREADS, 8) topk_distillation_grad_kernel(const __grid_constant__ DistillGradArgs p) {
     const int tid = threadIdx.x;
     const long long r = blockIdx.x / static_cast<unsigned>(p.chunks);
     const int V = p.rows.V;
@@ -1557,12 +1568,13 @@ __global__ void __launch_bounds__(THREADS, 4) topk_distillation_grad_kernel(cons
 }
 
 // ------------------------------------------------------------------ launches
-// CTAs per row: as many as fit on the GPU at once (three per SM) for all rows, while each keeps a step of work.  250 x 32000
-// fp32 logits, distillation forward: 13 us with one, 18 with two; 333 x 32000 bf16, scores: 9.1 with one, 12.2 with two.
+// CTAs per row: as many as fit on the GPU at once (six per SM) for all rows, while each keeps a step of work.  Beyond that
+// they only cost: 250 x 32000 fp32 logits, distillation forward, with CTAs of eight warps: 13 us with one, 18 with two; 333 x
+// 32000 bf16, scores: 9.1 and 12.2.
 inline int splits_for(long long rows, int V, int elem) {
     const int step = THREADS * 16 / elem;
     int n = 1;
-    while (n < MAX_SPLITS && rows * n * 2 <= 148 * 3 && V > step * n) n *= 2;
+    while (n < MAX_SPLITS && rows * n * 2 <= 148 * 6 && V > step * n) n *= 2;
     return n;
 }
 
@@ -1585,8 +1597,8 @@ inline cudaError_t launch(Kern kern, const Args& a, long long ctas, int splits, 
 inline bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 inline int elem_size(int dtype) { return dtype == LME_F32 ? 4 : 2; }
 // Steps of a gradient's CTA: eight where that still makes many CTAs, so that what it has to know of its row costs little, else
-// four, fewer where SMs would be idle.  Distillation at 8192 x 128256 bf16, backward: 656 us with eight, 668 with four, 741
-// with two; at 2047 x 50257: 82 with eight, 77 with four, 86 with two.
+// four, fewer where SMs would be idle (distillation at 8192 x 128256 bf16, backward: 644 us; sixteen steps: 674; at 2047 x
+// 50257: 78, with sixteen 76).
 struct GradGrid {
     int chunks, steps;
 };
@@ -1600,7 +1612,6 @@ inline GradGrid grad_grid(long long rows, int V, int elem) {
 }
 
 // Dynamic shared memory of the streaming kernels; the attribute is set to the most that any call asks for.
-constexpr int RING_STAGES = 2;
 constexpr int MAX_SMEM = ring_bytes(RING_STAGES) + MAX_MAP;
 template <typename T>
 inline cudaError_t launch_score(const ScoreArgs& a, long long ctas, void* stream) {

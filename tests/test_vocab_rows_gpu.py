@@ -718,3 +718,14 @@ def test_lists_that_hold_all_but_nothing(gap, method, tail):
     out = topk_distillation(leaf, ids[:, :3], lq[:, :3], None, method, tail)
     (g,) = torch.autograd.grad(out.kl_divergence.sum(), leaf)
     assert out.kl_divergence[0, 1].isnan() and g[0, 1].isnan().all() and g[0, 0].isfinite().all()
+
+
+@pytest.mark.parametrize("V,k,layout", [(15, 15, "odd start"), (32, 5, "pitch"), (64, 5, "dense"), (1187, 87, "odd start")])
+def test_alternatives_of_many_short_rows(V, k, layout):
+    """More rows than CTAs at once, their ends read element by element."""
+    from lm_engine_b200.ops import token_logprobs, token_logprobs_reference
+
+    x = _rows(1, 2500, V, BF, 3, layout)
+    want = token_logprobs_reference(x.double(), None, k).top_ids
+    for _ in range(50):
+        assert torch.equal(token_logprobs(x, None, top_k=k).top_ids, want)
