@@ -313,7 +313,9 @@ struct Ring {
                 for (int u = 0; u < UNROLL; ++u)
                     if (lane + 32 * u >= last) v[u] = Slice<T>::nothing();      // (and not what the slot held)
             f(step, v, whole);
-            // Only now: what a lane has used it has read.  (Requested right behind the reads, a stage was overwritten under them.)
+            // A bulk copy writes through the async proxy, which no barrier of the warp orders behind ordinary reads: every lane's
+            // fence does.  (Without one a stage that was requested right behind its reads was overwritten under them.)
+            fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) request(slot);
             if (++slot == stages) {
@@ -1319,7 +1321,6 @@ __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __g
                     else
                         asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(Elem<T>::NEG_INF) : "memory");
                 }
-                fence_proxy_async_smem();
             }
         },
         [&](int, uint4 (&v)[UNROLL], bool whole) {

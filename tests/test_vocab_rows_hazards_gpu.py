@@ -1,0 +1,42 @@
+"""Token log probabilities and distillation where parts of the kernels meet: stages of the ring that are filled again while
+rows take the careful steps."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _logits(rows, V, dtype, seed):
+    return (2 * torch.randn(1, rows, V, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,V", [(300, 50257), (1500, 12001)])
+def test_rows_with_forbidden_tokens_repeat_to_the_bit(rows, V, dtype):
+    """Minus infinity ends the tried steps: no branch then hangs on what a step adds before its stage is requested again.  A
+    stage that is overwritten under its reads changes sums from call to call, and against 64 bits."""
+    from lm_engine_b200.ops import token_logprobs, topk_distillation
+
+    x = _logits(rows, V, dtype, 5)
+    x[..., ::3] = -math.inf
+    lq, ids = torch.log_softmax(x.float(), -1).topk(9, -1)
+    lq = lq - 0.5
+    first = None
+    for _ in range(100):
+        s = token_logprobs(x, ids[..., 3], top_k=9, temperature=0.8)
+        d = topk_distillation(x, ids, lq, ids[..., 1], temperature=1.3)
+        got = [*s, *d]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+    best = x.sort(dim=-1, descending=True, stable=True).indices[..., :9]       # (topk orders equal ones as it likes)
+    assert torch.equal(first[3], best)
+    logp = torch.log_softmax(x.double() / 0.8, -1)
+    # a thread's sum of V / 128 exponentials, each off by 2^-22 and its exponent's rounding (24 nats: 2^-19), added in 32 bits
+    off = (V / 128 + 100) * 2.0 ** -24 + 2.0 ** -19
+    assert float((first[0] - logp.gather(-1, ids[..., 3:4])[..., 0]).abs().max()) < off
+    entropy = -(logp.exp() * logp.masked_fill(logp == -math.inf, 0.0)).sum(-1)
+    assert float((first[1] - entropy).abs().max()) < off * (2 + math.log2(V))
