@@ -295,8 +295,8 @@ struct Ring {
         return r;
     }
     // f(step, vectors, whether all of them are there) for every step; nothing behind the last whole vector.  first(step,
-    // address): before a lane reads its vectors, 512 bytes apart from `address` on.  After a wait that ran out the loop goes on
-    // without waiting (wrong rows, status word set).
+    // address): before a lane reads its vectors, 512 bytes apart from `address` on.  After a wait that ran out (status word set)
+    // the loop goes on with what the stages hold and requests nothing more; `ok` says that all has arrived.
     template <typename F0, typename F>
     __device__ __forceinline__ void stream(F0&& first, F&& f) {
         const int lane = threadIdx.x & 31;
@@ -317,16 +317,19 @@ struct Ring {
             // fence does.  (Without one a stage that was requested right behind its reads was overwritten under them.)
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) request(slot);
+            if (lane == 0 && ok) request(slot);
             if (++slot == stages) {
                 slot = 0;
                 phase ^= 1;
             }
         }
+        if (!ok) drain();
     }
-    // waits for what has been requested and not used: no copy may outlast its CTA
+    // Waits for what has been requested and not used: no copy may outlast its CTA.  Only the lane that requests knows how
+    // much that is; a slot's last request completes its phase number (ahead - 1 - slot) / stages.
     __device__ __forceinline__ void drain() {
-        for (int i = 0; i < min(stages, steps); ++i) wait(full + 8 * i, 0);
+        if ((threadIdx.x & 31) == 0)
+            for (int i = 0; i < min(stages, ahead); ++i) wait(full + 8 * i, (ahead - 1 - i) / stages & 1);
     }
 
 private:
@@ -527,13 +530,14 @@ struct Running {
         return true;
     }
 };
-// The CTA's sums, relative to its largest base, in every thread (`red`: 4 * WARPS floats).
+// The CTA's sums, relative to its largest base, in every thread (`red`: 4 * WARPS floats).  all_ok: a thread's answer becomes the
+// CTA's.
 struct Sums {
     float m;
     double s, w, s1;
 };
 template <bool ENTROPY, AtOne ONE>
-__device__ __forceinline__ Sums join_block(Running<ENTROPY, ONE> r, float c, float c1, float* red) {
+__device__ __forceinline__ Sums join_block(Running<ENTROPY, ONE> r, float c, float c1, float* red, bool* all_ok = nullptr) {
     if (ENTROPY) r.settle(c);
     else r.leave(c, c1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -541,7 +545,8 @@ __device__ __forceinline__ Sums join_block(Running<ENTROPY, ONE> r, float c, flo
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) red[warp] = m;
-    __syncthreads();
+    if (all_ok != nullptr) *all_ok = __syncthreads_and(*all_ok);
+    else __syncthreads();
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) m = max_nan(m, red[i]);
     if (!(m <= r.m)) r.raise(m, c, c1);
@@ -965,7 +970,8 @@ __global__ void __launch_bounds__(THREADS, 6) token_logprobs_kernel(const __grid
             mine = max_nan(mine, m);
         }
     }
-    Sums sum = join_block(run, c, 0.f, red);
+    bool arrived = ring.ok;             // if not, the ring's memory may still be written to and serves nothing else
+    Sums sum = join_block(run, c, 0.f, red, TOP ? &arrived : nullptr);
     // the row's last values: one thread of the last warp, while the others select
     auto finish = [&] {
         const double log_s = log(sum.s), entropy = log_s - sum.w / sum.s * LN2;
@@ -984,7 +990,8 @@ __global__ void __launch_bounds__(THREADS, 6) token_logprobs_kernel(const __grid
     };
     if (p.splits == 1 && tid == THREADS - 1) finish();
     int n = 0;
-    if constexpr (TOP) n = select_best<T>(sel, group, row, p.rows.V, rank, p.splits, p.k, mine, segment_shift);
+    if constexpr (TOP)
+        if (arrived) n = select_best<T>(sel, group, row, p.rows.V, rank, p.splits, p.k, mine, segment_shift);
 
     if (p.splits > 1) {
         if (tid == 0) {
@@ -1016,15 +1023,17 @@ __global__ void __launch_bounds__(THREADS, 6) token_logprobs_kernel(const __grid
             sum = Sums{m, __shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, w, 0), 0.0};
             if (tid == THREADS - 1) finish();
             if constexpr (TOP) {
-                int base = 0;
-                __syncthreads();
-                for (int q = 0; q < p.splits; ++q) {
-                    const int nb = __shfl_sync(0xffffffffu, nq, q);
-                    for (int i = tid; i < nb; i += THREADS) sel.cand[base + i] = ld_peer(&sel.best[i], q);
-                    base += nb;
+                if (arrived) {
+                    int base = 0;
+                    __syncthreads();
+                    for (int q = 0; q < p.splits; ++q) {
+                        const int nb = __shfl_sync(0xffffffffu, nq, q);
+                        for (int i = tid; i < nb; i += THREADS) sel.cand[base + i] = ld_peer(&sel.best[i], q);
+                        base += nb;
+                    }
+                    __syncthreads();
+                    n = order_candidates(sel, base, p.k);
                 }
-                __syncthreads();
-                n = order_candidates(sel, base, p.k);
             }
         }
     }
@@ -1036,6 +1045,9 @@ __global__ void __launch_bounds__(THREADS, 6) token_logprobs_kernel(const __grid
                 p.top_ids[r * p.k + tid] = index_of(b);
                 p.top_logprobs[r * p.k + tid] = static_cast<float>(
                     (static_cast<double>(value_of(static_cast<uint32_t>(b >> 32))) - sum.m) * p.inv_temperature - row_log_s);
+            } else if (tid < p.k) {     // (only where something has not arrived: an id that may be used as an index)
+                p.top_ids[r * p.k + tid] = 0;
+                p.top_logprobs[r * p.k + tid] = __int_as_float(0x7fffffff);
             }
         }
     }
