@@ -1313,9 +1313,13 @@ __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __g
         const int bit = (sl.whole(j) ? q % WARP_STEP / 32 * 8 : 0) + (id + sl.before) % N;
         again = atomicOr(&listed[word], 1u << bit) >> bit & 1u;
     }
-    bool counts = mine;
-    if (__syncthreads_or(again) && mine)
-        for (int i = 0; i < tid; ++i) counts &= id_of[i] != id;
+    // Only an id's first entry counts, also for the largest value, which is of the whole list and asked for without a tail: this
+    // CTA's map says nothing of ids in the others.
+    bool first = id >= 0;
+    if (__syncthreads_or(again) || (p.splits > 1 && !p.tail))
+        if (first)
+            for (int i = 0; i < tid; ++i) first &= id_of[i] != id;
+    const bool counts = mine && first;
     if (tid < p.k && (mine || (rank == 0 && id < 0))) p.entries[r * p.k + tid] = counts ? id : -1;
     const float x = counts ? Elem<T>::f(row[id]) : -INFINITY;
     const float x_label = rank == 0 && tid == 0 && labelled && label >= 0 && label < V ? Elem<T>::f(row[label]) : 0.f;
@@ -1348,7 +1352,7 @@ __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __g
     Sums sum = join_block(run, c, LOG2E, red);
 
     // the listed tokens, in 64 bits.  Weights without a tail are relative to the largest value of the list.
-    float m = max_nan(x, -INFINITY), ref = id >= 0 ? lq : -INFINITY;
+    float m = max_nan(x, -INFINITY), ref = first ? lq : -INFINITY;
     if (warp < MAX_K / 32) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {

@@ -1,5 +1,5 @@
 """Token log probabilities and distillation where parts of the kernels meet: stages of the ring that are filled again while
-rows take the careful steps."""
+rows take the careful steps, repeated entries of a teacher's list, upstream gradients that are not plain tensors."""
 
 import math
 
@@ -40,3 +40,31 @@ def test_rows_with_forbidden_tokens_repeat_to_the_bit(rows, V, dtype):
     assert float((first[0] - logp.gather(-1, ids[..., 3:4])[..., 0]).abs().max()) < off
     entropy = -(logp.exp() * logp.masked_fill(logp == -math.inf, 0.0)).sum(-1)
     assert float((first[1] - entropy).abs().max()) < off * (2 + math.log2(V))
+
+
+@pytest.mark.parametrize("rows", [2, 250, 900])
+@pytest.mark.parametrize("method,tail", [("backward", False), ("backward", True), ("forward", True)])
+@pytest.mark.parametrize("value", [900.0, -900.0, math.nan, math.inf])
+def test_values_of_repeated_entries_are_not_looked_at(rows, method, tail, value):
+    """One CTA or several per row (the entries of a token lie in one of them, the values' largest is of all)."""
+    from lm_engine_b200.ops import topk_distillation
+
+    V, K = 20000, 24
+    x = _logits(rows, V, F32, 3).requires_grad_(True)
+    lq, ids = (x.detach() + _logits(rows, V, F32, 4)).topk(K, -1)
+    if tail:
+        lq = torch.log_softmax(lq, -1) - 0.5
+    ids[..., 9], ids[..., 20] = ids[..., 2], ids[..., 17]
+    fewer = ids.clone()
+    fewer[..., 9] = fewer[..., 20] = -1
+    lq[..., 9] = lq[..., 20] = value
+    d = torch.rand(1, rows, device="cuda") + 0.5
+
+    def run(which):
+        kl = topk_distillation(x, which, lq, None, method, tail).kl_divergence
+        return kl, *torch.autograd.grad(kl, x, d)
+
+    (kl, g), (kl_fewer, g_fewer) = run(ids), run(fewer)
+    assert kl.isfinite().all()
+    # the same entries count: the same sums, whatever stands at the others
+    assert torch.equal(kl, kl_fewer) and torch.equal(g, g_fewer)
