@@ -35,12 +35,13 @@ def topk_distillation_reference(logits: torch.Tensor, top_ids: torch.Tensor, top
                                 kl_divergence_method: KLDivergenceMethod = KLDivergenceMethod.backward, tail: bool = True,
                                 temperature=1.0, ignore_index: int = -100) -> TopkDistillation:
     V = logits.size(-1)
+    top_ids, labels = top_ids.long(), None if labels is None else labels.long()    # (narrow types would compare modulo their range)
     teacher = top_logprobs.detach().double()
     there = (top_ids >= 0) & (top_ids < V) & (teacher != -torch.inf)
     same = (top_ids[..., :, None] == top_ids[..., None, :]) & there[..., None, :]
     there = there & ~same.tril(-1).any(-1)                      # an id's first entry counts
     asked = there.any(-1)
-    ids = torch.where(there, top_ids, 0).long()
+    ids = torch.where(there, top_ids, 0)
     x = logits if logits.dtype == torch.float64 else logits.float()
     if labels is None:
         read = asked
@@ -75,7 +76,7 @@ def topk_distillation_reference(logits: torch.Tensor, top_ids: torch.Tensor, top
     if labels is None:
         return TopkDistillation(kl, None)
     inside = (labels >= 0) & (labels < V)
-    nll = F.cross_entropy(x.reshape(-1, V), torch.where(inside, labels, 0).reshape(-1).long(),
+    nll = F.cross_entropy(x.reshape(-1, V), torch.where(inside, labels, 0).reshape(-1),
                           reduction="none").view(labels.shape)
     nll = torch.where(labels == ignore_index, 0.0, torch.where(inside, nll, float("nan")))
     return TopkDistillation(kl, nll)

@@ -33,8 +33,9 @@ def token_logprobs_reference(logits: torch.Tensor, tokens: torch.Tensor | None =
     logp = torch.log_softmax(x / temperature, -1)
     picked = top = ids = None
     if tokens is not None:
+        tokens = tokens.long()          # a narrow type would take the vocabulary and ignore_index modulo its range
         inside = (tokens >= 0) & (tokens < x.size(-1))
-        at = torch.where(inside, tokens, 0).long()
+        at = torch.where(inside, tokens, 0)
         picked = torch.where(inside, logp.gather(-1, at[..., None])[..., 0], float("nan"))
         picked = torch.where(tokens == ignore_index, 0.0, picked)
     p = logp.exp()
