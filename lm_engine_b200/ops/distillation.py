@@ -14,7 +14,8 @@ import torch.nn.functional as F
 
 from ..enums import KLDivergenceMethod
 from . import _lib
-from .logprobs import KERNEL_TYPES, MAX_TOP_K, as_int64, check_logits, check_tokens, integers, kernel_usable, logit_rows
+from .logprobs import (KERNEL_TYPES, MAX_TOP_K, as_int64, check_logits, check_tokens, integers, kernel_usable, logit_rows,
+                       plain, statement_gradient)
 
 #: The teacher's mass outside of its listed tokens is one minus their sum, which the rounding of fp32 log probabilities moves by
 #: about this much: a smaller rest counts as none, and as this much where its logarithm is asked for.
@@ -115,11 +116,10 @@ class _TopkDistillation(torch.autograd.Function):
         nothing = (None,) * 7
         if d_kl is None and d_nll is None:
             return None, *nothing
-        if torch.is_grad_enabled():         # a graph of the gradients is asked for
-            x = logits.view_as(logits)
-            outs = topk_distillation_reference(x, top_ids, top_logprobs, labels, method, tail, temperature, ignore_index)
-            outs, grads = zip(*((o, g) for o, g in zip(outs, (d_kl, d_nll)) if g is not None))
-            return *torch.autograd.grad(outs, [x], grads, create_graph=True), *nothing
+        if torch.is_grad_enabled() or not plain(d_kl, d_nll):
+            return statement_gradient(
+                logits, lambda x: topk_distillation_reference(x, top_ids, top_logprobs, labels, method, tail, temperature,
+                                                              ignore_index), (d_kl, d_nll)), *nothing
         x, inner, ld_inner, ld_outer = logit_rows(logits)
         V = x.size(-1)
         top_logprobs, labels, d_kl, d_nll = (None if t is None else t.contiguous()

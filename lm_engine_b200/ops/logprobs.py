@@ -97,6 +97,25 @@ def check_tokens(name: str, tokens: torch.Tensor, logits: torch.Tensor) -> None:
                          f"{tuple(tokens.shape)}")
 
 
+_is_batched = torch._C._functorch.is_legacy_batchedtensor
+
+
+def plain(*upstream: torch.Tensor | None) -> bool:
+    """Whether kernels may take upstream gradients by address.  Those of ``autograd.grad(is_grads_batched=True)`` are batched by a
+    mechanism of their own, which no interpreter stack shows."""
+    return _lib.eager(*upstream) and not any(t is not None and _is_batched(t) for t in upstream)
+
+
+def statement_gradient(logits, statement, upstream):
+    """Gradient of the logits by the PyTorch operations: where a graph of it is asked for, or where the upstream values are not
+    plain tensors (a vmap over the backward pass)."""
+    graph = torch.is_grad_enabled()
+    with torch.enable_grad():
+        x = logits.view_as(logits)
+        outs, grads = zip(*((o, g) for o, g in zip(statement(x), upstream) if g is not None))
+        return torch.autograd.grad(outs, [x], grads, create_graph=graph)[0]
+
+
 def _forward(logits, tokens, top_k, temperature, ignore_index, with_stats):
     x, inner, ld_inner, ld_outer = logit_rows(logits)
     shape = x.shape
@@ -141,11 +160,11 @@ class _TokenLogprobs(torch.autograd.Function):
         top_k, temperature, ignore_index = ctx.meta
         if d_logprobs is None and d_entropy is None and d_top is None:
             return None, None, None, None, None
-        if torch.is_grad_enabled():         # a graph of the gradients is asked for
-            x = logits.view_as(logits)
-            outs = token_logprobs_reference(x, tokens, top_k, temperature, ignore_index)[:3]
-            outs, grads = zip(*((o, g) for o, g in zip(outs, (d_logprobs, d_entropy, d_top)) if g is not None))
-            return *torch.autograd.grad(outs, [x], grads, create_graph=True), None, None, None, None
+        if torch.is_grad_enabled() or not plain(d_logprobs, d_entropy, d_top):
+            grad = statement_gradient(
+                logits, lambda x: token_logprobs_reference(x, tokens, top_k, temperature, ignore_index)[:3],
+                (d_logprobs, d_entropy, d_top))
+            return grad, None, None, None, None
         x, inner, ld_inner, ld_outer = logit_rows(logits)
         V = x.size(-1)
         small = [None if t is None else t.contiguous() for t in (tokens, ids, d_logprobs, d_entropy, d_top)]

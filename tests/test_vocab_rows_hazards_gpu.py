@@ -68,3 +68,33 @@ def test_values_of_repeated_entries_are_not_looked_at(rows, method, tail, value)
     assert kl.isfinite().all()
     # the same entries count: the same sums, whatever stands at the others
     assert torch.equal(kl, kl_fewer) and torch.equal(g, g_fewer)
+
+
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_batched_upstream_gradients(create_graph):
+    """Upstream values of a vmap over the backward pass have no memory of their own: the PyTorch operations take them."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from lm_engine_b200.ops import _lib, token_logprobs, topk_distillation
+
+    rows, V = 6, 300
+    x = _logits(rows, V, F32, 7).requires_grad_(True)
+    lq, ids = torch.log_softmax(x.detach(), -1).topk(5, -1)
+    lq = lq - 0.5
+    s, d = token_logprobs(x, ids[..., 2], top_k=3, temperature=0.7), topk_distillation(x, ids, lq, ids[..., 1], temperature=1.5)
+    for out in (s.logprobs, s.entropy, s.top_logprobs, d.kl_divergence, d.nll):
+        up = torch.eye(out.numel(), device="cuda").view(-1, *out.shape)
+        (all_at_once,) = torch.autograd.grad([out], [x], [up], is_grads_batched=True, retain_graph=True, create_graph=create_graph)
+        assert all_at_once.requires_grad == create_graph
+        before = _lib.launch_count
+        one_by_one = torch.stack([torch.autograd.grad([out], [x], [u], retain_graph=True)[0] for u in up])
+        assert _lib.launch_count == before + len(up)
+        # both fp32, of sums of 300 exponentials: (300 / 128 + 100) 2^-24 relatively, on terms that add up to at most 2 / 0.7
+        # times 1 + |log p| <= 16; entropies' twice
+        assert float((all_at_once.detach() - one_by_one).abs().max()) < 104 * 2.0 ** -24 * 2 * 3 * 16
+    j = torch.autograd.functional.jacobian(lambda v: token_logprobs(v, ids[..., 2]).logprobs, x.detach(), vectorize=True)
+    assert j.shape == (1, rows, 1, rows, V) and j.isfinite().all()
+    with FlopCounterMode(display=False):
+        (g,) = torch.autograd.grad([d.kl_divergence.sum()], [x], retain_graph=True)
+    (h,) = torch.autograd.grad([d.kl_divergence.sum()], [x])
+    assert float((g - h).abs().max()) < 104 * 2.0 ** -24 * 3 * 16
