@@ -25,6 +25,7 @@ constexpr int WARPS = THREADS / 32;
 constexpr int UNROLL = 4;               // vectors of 16 bytes per thread and step
 constexpr int WARP_STEP = 32 * UNROLL;  // vectors of a warp and step
 constexpr int RING_STAGES = 2;
+constexpr int RING_BYTES = WARPS * RING_STAGES * WARP_STEP * 16;
 constexpr int MAX_SPLITS = 8;           // CTAs of a cluster
 constexpr int MAX_K = LME_VOCAB_MAX_K;  // best tokens, or tokens of a teacher, per row
 constexpr int SEGMENTS = 16;            // of a CTA's steps: what the selection reads again goes by their maxima
@@ -141,8 +142,6 @@ template <>
 struct Elem<float> {
     static constexpr int N = 4;
     static constexpr uint32_t NEG_INF = 0xff800000u;
-    static constexpr uint32_t LOW2 = 0;
-    static constexpr float LOW = 0.f;                   // (one value per word: nothing is gained)
     static __device__ __forceinline__ float f(float x) { return x; }
     static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
         f[0] = __uint_as_float(u.x);
@@ -243,13 +242,9 @@ struct Slice {
     __device__ __forceinline__ bool whole(int j) const { return j >= full0 && j < full1; }
     __device__ __forceinline__ uint4 load_any(int j) const { return whole(j) ? load(j) : load_part(j); }
     __device__ __forceinline__ int steps() const { return (full1 - full0 + THREADS * UNROLL - 1) / (THREADS * UNROLL); }
-    // this thread's vectors of a step: j, j + 32, ...
-    __device__ __forceinline__ int first(int step) const {
-        return full0 + step * (THREADS * UNROLL) + static_cast<int>(threadIdx.x >> 5) * WARP_STEP + static_cast<int>(threadIdx.x & 31);
-    }
 };
 
-// A warp's whole vectors arrive in a ring of its own, `stages` steps of 2 KB that one lane requests ahead: the loads in
+// A warp's whole vectors arrive in a ring of its own, two steps of 2 KB that one lane requests ahead: the loads in
 // flight take no registers, and no warp waits for another.
 template <typename T>
 struct Ring {
@@ -258,24 +253,24 @@ struct Ring {
     // they had been used for the last time, they came back over what was stored
     uint32_t buf, full;
     const T* source;        // of the next request
-    int stages, steps;      // steps: those in which this warp has vectors
+    int steps;              // those in which this warp has vectors
     int last;               // vectors of the last one
     int ahead;              // requests so far
     bool ok;
 
-    __device__ __forceinline__ Ring(const Slice<T>& sl, uint8_t* smem, uint64_t* barriers, int stages_) : stages(stages_), ahead(0), ok(true) {
+    __device__ __forceinline__ Ring(const Slice<T>& sl, uint8_t* smem, uint64_t* barriers) : ahead(0), ok(true) {
         const int warp = threadIdx.x >> 5;
-        buf = smem_u32(smem) + warp * stages * BYTES;
-        uint64_t* bars = barriers + warp * stages;
+        buf = smem_u32(smem) + warp * RING_STAGES * BYTES;
+        uint64_t* bars = barriers + warp * RING_STAGES;
         full = smem_u32(bars);
         const int j = sl.full0 + warp * WARP_STEP;
         steps = j < sl.full1 ? (sl.full1 - j - 1) / (THREADS * UNROLL) + 1 : 0;
         last = min(WARP_STEP, sl.full1 - j - (steps - 1) * (THREADS * UNROLL));
         source = sl.at(j);
         if ((threadIdx.x & 31) == 0) {
-            for (int i = 0; i < stages; ++i) mbar_init(bars + i, 1);
+            for (int i = 0; i < RING_STAGES; ++i) mbar_init(bars + i, 1);
             fence_barrier_init();
-            for (int i = 0; i < stages; ++i) request(i);
+            for (int i = 0; i < RING_STAGES; ++i) request(i);
         }
         __syncwarp();
     }
@@ -318,7 +313,7 @@ struct Ring {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && ok) request(slot);
-            if (++slot == stages) {
+            if (++slot == RING_STAGES) {
                 slot = 0;
                 phase ^= 1;
             }
@@ -326,10 +321,10 @@ struct Ring {
         if (!ok) drain();
     }
     // Waits for what has been requested and not used: no copy may outlast its CTA.  Only the lane that requests knows how
-    // much that is; a slot's last request completes its phase number (ahead - 1 - slot) / stages.
+    // much that is; a slot's last request completes its phase number (ahead - 1 - slot) / RING_STAGES.
     __device__ __forceinline__ void drain() {
         if ((threadIdx.x & 31) == 0)
-            for (int i = 0; i < min(stages, ahead); ++i) wait(full + 8 * i, (ahead - 1 - i) / stages & 1);
+            for (int i = 0; i < min(RING_STAGES, ahead); ++i) wait(full + 8 * i, (ahead - 1 - i) / RING_STAGES & 1);
     }
 
 private:
@@ -362,8 +357,6 @@ __device__ __forceinline__ float max_of(const uint4 (&r)[U]) {
     return Elem<T>::max_halves(w);
 }
 
-__host__ __device__ constexpr int ring_bytes(int stages) { return WARPS * stages * WARP_STEP * 16; }
-
 // ------------------------------------------------------------------ running sums of a thread
 // m: a base that no logit so far is above by more than SLACK / c, s: sum of 2^t, w: sum of 2^t t with t = (x - m) c.  The base
 // follows the largest logit only past the slack: a thread meets a new largest in most of its steps at first, and its warp with
@@ -387,7 +380,7 @@ struct Running {
     // temperature 0.8: off by 1.1e-5 on average, so by 2e-7; 2 to 3 % of the time).
     float s = 0.f, w = 0.f, s_lost = 0.f, w_lost = 0.f;
     float s1 = 0.f;                 // s at temperature one (c1)
-    bool far = false;               // LOW is so far below the base that it counts nothing
+    bool far = false;               // 16-bit types: LOW is so far below the base that it counts nothing
     bool trying = false, tried = false;
     float n = 0.f, n1 = 0.f;        // while trying
 
@@ -465,13 +458,18 @@ struct Running {
         const float x = largest();
         if (!(x <= limit)) {
             raise(x, c, c1);
-            far = m - Elem<T>::LOW > __fdividef(200.f, c) && c < 1e8f;
+            if constexpr (Elem<T>::N == 8) far = m - Elem<T>::LOW > __fdividef(200.f, c) && c < 1e8f;
         }
         // 0 * (-inf) must not get into w: a limit on t costs an instruction per logit, one on the packed logits half of one, and
-        // serves where what it turns a logit into is zero too
-        if (!ENTROPY) sum<T, U, false, false, false>(r, c, c1);
-        else if (Elem<T>::N == 8 && far) sum<T, U, false, true, false>(r, c, c1);
-        else sum<T, U, false, false, true>(r, c, c1);
+        // serves where what it turns a logit into is zero too (of fp32 there is one per word: nothing is gained)
+        if constexpr (!ENTROPY) {
+            sum<T, U, false, false, false>(r, c, c1);
+        } else if constexpr (Elem<T>::N == 8) {
+            if (far) sum<T, U, false, true, false>(r, c, c1);
+            else sum<T, U, false, false, true>(r, c, c1);
+        } else {
+            sum<T, U, false, false, true>(r, c, c1);
+        }
         if (!tried) enter(c, c1);
     }
     // false, and nothing added, where a try has run over
@@ -484,7 +482,7 @@ struct Running {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             uint4 v = r[u];
-            if (LIMIT_X) {
+            if constexpr (LIMIT_X) {
                 constexpr uint32_t low = Elem<T>::LOW2;
                 v = make_uint4(Elem<T>::max2(v.x, low), Elem<T>::max2(v.y, low), Elem<T>::max2(v.z, low), Elem<T>::max2(v.w, low));
             }
@@ -901,7 +899,7 @@ struct ScoreArgs {
     const long long* tokens;        // or null
     long long ignore_index;
     double inv_temperature;
-    int k, splits, stages;
+    int k, splits;
     float *logprobs, *entropy, *top_logprobs;
     long long* top_ids;
     float* stats;                   // [rows][4]: m, S, entropy, log S; or null
@@ -929,7 +927,7 @@ __global__ void __launch_bounds__(THREADS, 6) token_logprobs_kernel(const __grid
     const Slice<T> sl(row, p.rows.V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
 
-    Ring<T> ring(sl, vocab_smem, ring_bars, p.stages);
+    Ring<T> ring(sl, vocab_smem, ring_bars);
     long long tok = 0;              // of the thread that finishes the row
     float x_tok = 0.f;
     if (p.tokens != nullptr && rank == 0 && tid == THREADS - 1) {
@@ -1237,7 +1235,7 @@ struct DistillArgs {
     const long long* labels;        // or null
     long long ignore_index;
     double inv_temperature;
-    int k, splits, stages, forward_kl, tail;
+    int k, splits, forward_kl, tail;
     float *kl, *nll;
     int* entries;                   // [rows][k]: the ids that count, -1 elsewhere
     float* stats;                   // [rows][12]
@@ -1261,7 +1259,7 @@ template <typename T, AtOne ONE>
 __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
     constexpr int N = Elem<T>::N;
     extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then the map
-    uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + ring_bytes(p.stages));
+    uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + RING_BYTES);
     __shared__ float red[4 * WARPS];
     __shared__ uint64_t ring_bars[WARPS * RING_STAGES];
     __shared__ int id_of[MAX_K];
@@ -1277,7 +1275,7 @@ __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __g
     const Slice<T> sl(row, V, rank, p.splits);
     const float c = static_cast<float>(p.inv_temperature * 1.4426950408889634);
 
-    Ring<T> ring(sl, vocab_smem, ring_bars, p.stages);
+    Ring<T> ring(sl, vocab_smem, ring_bars);
     // the list: entries that count are in the vocabulary, have a finite or NaN value, and come first of their token
     static_assert(UNROLL == 4, "a word of the map has a lane's vectors of a step");
     const int words = (sl.full1 - sl.full0 + WARP_STEP - 1) / WARP_STEP * 32;       // and one each for the parts at the ends
@@ -1353,45 +1351,42 @@ __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __g
 
     // the listed tokens, in 64 bits.  Weights without a tail are relative to the largest value of the list.
     float m = max_nan(x, -INFINITY), ref = first ? lq : -INFINITY;
-    if (warp < MAX_K / 32) {
+    static_assert(MAX_K == THREADS, "every warp has a part of the list");
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-            ref = max_nan(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-        }
-        if (lane == 0) {
-            list_max[0][warp] = m;
-            list_max[1][warp] = ref;
-        }
+    for (int o = 16; o > 0; o >>= 1) {
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        ref = max_nan(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+    }
+    if (lane == 0) {
+        list_max[0][warp] = m;
+        list_max[1][warp] = ref;
     }
     __syncthreads();
-    if (warp < MAX_K / 32) {
 #pragma unroll
-        for (int i = 0; i < MAX_K / 32; ++i) {
-            m = max_nan(m, list_max[0][i]);
-            ref = max_nan(ref, list_max[1][i]);
-        }
-        m = max_nan(m, sum.m);
-        if (p.tail || ref == -INFINITY) ref = 0.f;
-        double e[4] = {0, 0, 0, 0};     // listed exponentials, at temperature one, weights, products
-        if (counts) {
-            const double d = static_cast<double>(x) - m, y = static_cast<double>(x) * p.inv_temperature;
-            e[0] = x == -INFINITY ? 0.0 : exp(d * p.inv_temperature);
-            if (ONE) e[1] = x == -INFINITY ? 0.0 : exp(d);
-            e[2] = exp(static_cast<double>(lq) - ref);
-            if (p.forward_kl) e[3] = e[0] == 0.0 ? 0.0 : e[0] * (y - lq);
-            else e[3] = e[2] == 0.0 ? 0.0 : e[2] * (static_cast<double>(lq) - ref - y);
-        }
-        if (p.k > 32 * warp) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (ONE || q != 1)
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) e[q] += __shfl_xor_sync(0xffffffffu, e[q], o);
-        }
-        if (lane == 0)
-            for (int q = 0; q < 4; ++q) part_of[warp][q] = e[q];
+    for (int i = 0; i < MAX_K / 32; ++i) {
+        m = max_nan(m, list_max[0][i]);
+        ref = max_nan(ref, list_max[1][i]);
     }
+    m = max_nan(m, sum.m);
+    if (p.tail || ref == -INFINITY) ref = 0.f;
+    double e[4] = {0, 0, 0, 0};     // listed exponentials, at temperature one, weights, products
+    if (counts) {
+        const double d = static_cast<double>(x) - m, y = static_cast<double>(x) * p.inv_temperature;
+        e[0] = x == -INFINITY ? 0.0 : exp(d * p.inv_temperature);
+        if (ONE) e[1] = x == -INFINITY ? 0.0 : exp(d);
+        e[2] = exp(static_cast<double>(lq) - ref);
+        if (p.forward_kl) e[3] = e[0] == 0.0 ? 0.0 : e[0] * (y - lq);
+        else e[3] = e[2] == 0.0 ? 0.0 : e[2] * (static_cast<double>(lq) - ref - y);
+    }
+    if (p.k > 32 * warp) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (ONE || q != 1)
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) e[q] += __shfl_xor_sync(0xffffffffu, e[q], o);
+    }
+    if (lane == 0)
+        for (int q = 0; q < 4; ++q) part_of[warp][q] = e[q];
     const int n = __syncthreads_count(counts);
     if (warp > 0 && p.splits == 1) return;
     if (tid == 0) {
@@ -1629,11 +1624,11 @@ inline GradGrid grad_grid(long long rows, int V, int elem) {
 }
 
 // Dynamic shared memory of the streaming kernels; the attribute is set to the most that any call asks for.
-constexpr int MAX_SMEM = ring_bytes(RING_STAGES) + MAX_MAP;
+constexpr int MAX_SMEM = RING_BYTES + MAX_MAP;
 template <typename T>
 inline cudaError_t launch_score(const ScoreArgs& a, long long ctas, void* stream) {
     const bool top = a.k > 0;
-    const int smem = max(ring_bytes(a.stages), top ? static_cast<int>(sizeof(Selection)) : 0);
+    const int smem = max(RING_BYTES, top ? static_cast<int>(sizeof(Selection)) : 0);
     if (!(top ? opt_in<token_logprobs_kernel<T, true>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM)
               : opt_in<token_logprobs_kernel<T, false>>(cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM)))
         return cudaErrorInvalidValue;
@@ -1661,7 +1656,7 @@ extern "C" int lme_token_logprobs_fwd(const void* x, int dtype, long long rows, 
         (k > 0 && (top_logprobs == nullptr || top_ids == nullptr)))
         return LME_ERR_SHAPE;
     if (misaligned(stats)) return LME_ERR_ALIGN;
-    const ScoreArgs a{{x, inner, ld_inner, ld_outer, V}, tokens, ignore_index, 1.0 / temperature, k, splits, RING_STAGES, logprobs, entropy,
+    const ScoreArgs a{{x, inner, ld_inner, ld_outer, V}, tokens, ignore_index, 1.0 / temperature, k, splits, logprobs, entropy,
                       top_logprobs, top_ids, stats};
     const long long ctas = rows * splits;
     const cudaError_t e = dtype == LME_BF16  ? launch_score<__nv_bfloat16>(a, ctas, stream)
@@ -1736,10 +1731,10 @@ extern "C" int lme_topk_distillation_fwd(const void* x, int dtype, long long row
         return LME_ERR_SHAPE;
     if (misaligned(stats)) return LME_ERR_ALIGN;
     const DistillArgs a{{x, inner, ld_inner, ld_outer, V}, top_ids, top_logprobs, labels, ignore_index, 1.0 / temperature, k,
-                        splits, RING_STAGES, forward_kl, tail, kl, nll, entries, stats};
+                        splits, forward_kl, tail, kl, nll, entries, stats};
     const AtOne one = at_one(labels != nullptr, temperature);
     const long long ctas = rows * splits;
-    const int smem = ring_bytes(a.stages) + map_bytes(splits);
+    const int smem = RING_BYTES + map_bytes(splits);
     const cudaError_t e = dtype == LME_BF16  ? launch_distill<__nv_bfloat16>(a, one, ctas, smem, stream)
                           : dtype == LME_F16 ? launch_distill<__half>(a, one, ctas, smem, stream)
                                              : launch_distill<float>(a, one, ctas, smem, stream);
