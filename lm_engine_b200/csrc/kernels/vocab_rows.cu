@@ -768,15 +768,16 @@ __device__ __forceinline__ void pick_bin(Selection& sel, int need) {
     }
 }
 
-// A value that at least k of the threads' largest values reach and hardly more do, into sel.reach: the edge of the bin of a
-// histogram in which the k-th falls.  Where too many fall into it (values of masked vocabularies or outliers stretch the bins,
-// values are equal) the k-th is found by the bits of its key, eight at a time.  NaN, which compares as reached, where fewer than k
-// threads have anything.
-__device__ __forceinline__ void find_reach(Selection& sel, float largest, int k) {
+// A value that at least k of the threads' largest values (two per thread) reach and hardly more do, into sel.reach: the edge of the
+// bin of a histogram in which the k-th falls.  Where too many fall into it (values of masked vocabularies or outliers stretch the
+// bins, values are equal) the k-th is found by the bits of its key, eight at a time.  NaN, which compares as reached, where there
+// are fewer than k.
+__device__ __forceinline__ void find_reach(Selection& sel, const float (&largest)[2], int k) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool some = !(largest == -INFINITY);          // (no vectors, or nothing but -inf: not counted)
-    const uint32_t key = key_of(largest);
-    const uint32_t hi = __reduce_max_sync(0xffffffffu, key), lo = __reduce_min_sync(0xffffffffu, some ? key : 0xffffffffu);
+    const bool some[2] = {!(largest[0] == -INFINITY), !(largest[1] == -INFINITY)};      // (no vectors, or nothing but -inf: not counted)
+    const uint32_t key[2] = {key_of(largest[0]), key_of(largest[1])};
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, max(key[0], key[1]));
+    const uint32_t lo = __reduce_min_sync(0xffffffffu, min(some[0] ? key[0] : 0xffffffffu, some[1] ? key[1] : 0xffffffffu));
     if (lane == 0) {
         sel.hi[warp] = hi;
         sel.lo[warp] = lo;
@@ -790,7 +791,9 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
         bottom = min(bottom, sel.lo[i]);
     }
     const float from = value_of(bottom), scale = __fdividef(BINS - 0.01f, value_of(top) - from);    // (0 or NaN: one bin)
-    if (some) atomicAdd(&sel.bin[min(BINS - 1, max(0, static_cast<int>((largest - from) * scale)))], 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (some[h]) atomicAdd(&sel.bin[min(BINS - 1, max(0, static_cast<int>((largest[h] - from) * scale)))], 1);
     __syncthreads();
     if (warp == 0) {
         pick_bin(sel, k);
@@ -810,7 +813,9 @@ __device__ __forceinline__ void find_reach(Selection& sel, float largest, int k)
         for (int shift = 24; shift >= 0; shift -= 8) {
             for (int i = tid; i < BINS; i += THREADS) sel.bin[i] = 0;
             __syncthreads();
-            if (some && (shift == 24 || key >> (shift + 8) == prefix)) atomicAdd(&sel.bin[key >> shift & 255], 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (some[h] && (shift == 24 || key[h] >> (shift + 8) == prefix)) atomicAdd(&sel.bin[key[h] >> shift & 255], 1);
             __syncthreads();
             if (warp == 0) pick_bin(sel, need);
             __syncthreads();
@@ -832,7 +837,16 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
     constexpr int N = Elem<T>::N, AHEAD = 4;
     const Slice<T> sl(row, V, rank, splits);
     const int tid = threadIdx.x;
-    find_reach(sel, largest, k);
+    // Nearly as many as there are threads: the smallest of their largest values say little (the k-th of 128 is reached by 700
+    // values for k = 128, and by more than there is room for in every twentieth row).  Odd and even segments by themselves make
+    // twice as many.
+    float halves[2] = {largest, -INFINITY};
+    if (k > THREADS / 2) {
+        halves[0] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < SEGMENTS + 1; ++i) halves[i & 1] = max_nan(halves[i & 1], group[i * THREADS + tid]);
+    }
+    find_reach(sel, halves, k);
     const float reach = sel.reach;
     if (!(largest < reach)) {
         uint32_t mask = 0;

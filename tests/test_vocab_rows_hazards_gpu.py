@@ -98,3 +98,50 @@ def test_batched_upstream_gradients(create_graph):
         (g,) = torch.autograd.grad([d.kl_divergence.sum()], [x], retain_graph=True)
     (h,) = torch.autograd.grad([d.kl_divergence.sum()], [x])
     assert float((g - h).abs().max()) < 104 * 2.0 ** -24 * 3 * 16
+
+
+def _time(run):
+    run()
+    best = math.inf
+    for _ in range(5):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        for _ in range(3):
+            run()
+        end.record()
+        end.synchronize()
+        best = min(best, start.elapsed_time(end))
+    return best
+
+
+def test_the_most_alternatives_of_ordinary_rows_are_selected_from_few():
+    """Nearly as many alternatives as a CTA has threads: rows whose candidates do not fit are read some thirty times more,
+    which one row in twenty is enough to show."""
+    from lm_engine_b200.ops import token_logprobs
+
+    x = _logits(2048, 128256, BF, 13)
+    want = x[0, :8].sort(dim=-1, descending=True, stable=True).indices
+    few = _time(lambda: token_logprobs(x, top_k=64))
+    for k in (65, 100, 127, 128):
+        assert torch.equal(token_logprobs(x, top_k=k).top_ids[0, :8], want[:, :k])
+        assert _time(lambda: token_logprobs(x, top_k=k)) < 3 * few          # (measured: 1.1 to 1.6; 16 with such rows)
+
+
+@pytest.mark.parametrize("rows", [1, 500])
+@pytest.mark.parametrize("V", [130, 1500, 4096, 8200, 8300, 33000])
+@pytest.mark.parametrize("k", [64, 65, 128])
+def test_alternatives_of_few_and_odd_segments(rows, V, k):
+    from lm_engine_b200.ops import token_logprobs
+
+    for dtype in (BF, F32):
+        x = _logits(rows, V, dtype, V)
+        for variant in range(4):
+            y = x.clone()
+            if variant == 1:
+                y[..., V // 3:] = -math.inf
+            elif variant == 2:
+                y[..., ::2] = math.nan
+            elif variant == 3:
+                y[..., : V - k] -= 100.0                # the best lie at the row's end, in the last segment
+            want = y.sort(dim=-1, descending=True, stable=True).indices[..., :k]
+            assert torch.equal(token_logprobs(y, top_k=k).top_ids, want)
