@@ -50,7 +50,7 @@ def topk_distillation_reference(logits: torch.Tensor, top_ids: torch.Tensor, top
         read = asked | (labels != ignore_index)
     x = torch.where(read[..., None], x, 0.0)                    # other rows are not looked at
     logp = torch.log_softmax(x / temperature, -1)
-    listed = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add_(-1, ids, there.int()) > 0
+    listed = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add(-1, ids, there.int()) > 0
     others = logp.double().masked_fill(listed, -torch.inf)      # in the logarithm: they may be less likely than a number can say
     none = (others == -torch.inf).all(-1)
     log_rest = torch.where(none, -torch.inf, others.masked_fill(none[..., None], 0.0).logsumexp(-1))

@@ -1,5 +1,5 @@
 """Ids of every integer type, on the PyTorch operations: compared with the vocabulary and the ignored index as numbers, not
-in their own type."""
+in their own type.  And transforms, which take the PyTorch operations too."""
 
 import math
 
@@ -60,3 +60,22 @@ def test_labels_and_lists_beside_the_ignored_index():
     want = topk_distillation(x, ids.long(), lq, labels.long())
     assert torch.equal(out.kl_divergence, want.kl_divergence) and torch.equal(out.nll, want.nll)
     assert out.kl_divergence[1] == 0 and float(out.nll[0]) > 0
+
+
+@pytest.mark.parametrize("method,tail", [("backward", True), ("backward", False), ("forward", True)])
+def test_transforms_over_positions(method, tail):
+    """vmap over positions, gradients position by position, and a derivative along a direction."""
+    x = _logits(40)
+    ids, labels = torch.tensor([[1, 2], [9, 7], [12, -1], [0, 27]]), torch.tensor([5, 10, -100, 0])
+    lq = torch.log(torch.rand(4, 2, generator=torch.Generator().manual_seed(2)) / 2)
+    want = topk_distillation(x, ids, lq, labels, method, tail)
+    one = lambda v, i, q, t: topk_distillation(v, i, q, t, method, tail)        # noqa: E731
+    got = torch.func.vmap(one)(x, ids, lq, labels)
+    assert torch.allclose(got.kl_divergence, want.kl_divergence) and torch.allclose(got.nll, want.nll)
+    per = torch.func.vmap(torch.func.grad(lambda *a: sum(one(*a))))(x, ids, lq, labels)
+    leaf = x.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(sum(o.sum() for o in one(leaf, ids, lq, labels)), leaf)
+    assert torch.allclose(per, g)
+    along = torch.randn(x.shape, generator=torch.Generator().manual_seed(3), dtype=x.dtype)
+    _, d = torch.func.jvp(lambda v: sum(o.sum() for o in one(v, ids, lq, labels)), (x,), (along,))
+    assert torch.allclose(d, (g * along).sum())
