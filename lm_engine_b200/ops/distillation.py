@@ -15,7 +15,7 @@ import torch.nn.functional as F
 from ..enums import KLDivergenceMethod
 from . import _lib
 from .logprobs import (KERNEL_TYPES, MAX_TOP_K, as_int64, check_logits, check_tokens, integers, kernel_usable, logit_rows,
-                       plain, statement_gradient)
+                       statement_gradient)
 
 #: The teacher's mass outside of its listed tokens is one minus their sum, which the rounding of fp32 log probabilities moves by
 #: about this much: a smaller rest counts as none, and as this much where its logarithm is asked for.
@@ -116,20 +116,22 @@ class _TopkDistillation(torch.autograd.Function):
         nothing = (None,) * 7
         if d_kl is None and d_nll is None:
             return None, *nothing
-        if torch.is_grad_enabled() or not plain(d_kl, d_nll):
+        small = [None if t is None else t.contiguous() for t in (top_logprobs, labels, d_kl, d_nll)]
+        try:
+            at = None if torch.is_grad_enabled() else [_lib.ptr(t) for t in small]
+        except RuntimeError:                # upstream values without an address
+            at = None
+        if at is None:
             return statement_gradient(
                 logits, lambda x: topk_distillation_reference(x, top_ids, top_logprobs, labels, method, tail, temperature,
                                                               ignore_index), (d_kl, d_nll)), *nothing
         x, inner, ld_inner, ld_outer = logit_rows(logits)
         V = x.size(-1)
-        top_logprobs, labels, d_kl, d_nll = (None if t is None else t.contiguous()
-                                             for t in (top_logprobs, labels, d_kl, d_nll))
         grad = torch.empty_like(x, memory_format=torch.contiguous_format)
         rc = _lib.cuda_lib().lme_topk_distillation_bwd(
             x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // V, inner, ld_inner, ld_outer, V, ctx.entries.data_ptr(),
-            top_logprobs.data_ptr(), top_ids.size(-1), _lib.ptr(labels), ignore_index, temperature,
-            method is KLDivergenceMethod.forward, ctx.stats.data_ptr(), _lib.ptr(d_kl), _lib.ptr(d_nll),
-            grad.data_ptr(), _lib.stream_ptr())
+            at[0], top_ids.size(-1), at[1], ignore_index, temperature, method is KLDivergenceMethod.forward,
+            ctx.stats.data_ptr(), at[2], at[3], grad.data_ptr(), _lib.stream_ptr())
         if rc:
             _lib.check(rc, "lme_topk_distillation_bwd")
         _lib.count_launch()

@@ -97,18 +97,9 @@ def check_tokens(name: str, tokens: torch.Tensor, logits: torch.Tensor) -> None:
                          f"{tuple(tokens.shape)}")
 
 
-_is_batched = torch._C._functorch.is_legacy_batchedtensor
-
-
-def plain(*upstream: torch.Tensor | None) -> bool:
-    """Whether kernels may take upstream gradients by address.  Those of ``autograd.grad(is_grads_batched=True)`` are batched by a
-    mechanism of their own, which no interpreter stack shows."""
-    return _lib.eager(*upstream) and not any(t is not None and _is_batched(t) for t in upstream)
-
-
 def statement_gradient(logits, statement, upstream):
-    """Gradient of the logits by the PyTorch operations: where a graph of it is asked for, or where the upstream values are not
-    plain tensors (a vmap over the backward pass)."""
+    """Gradient of the logits by the PyTorch operations: where a graph of it is asked for, or where the upstream values have no
+    address (in a vmap over the backward pass, so with ``autograd.grad(is_grads_batched=True)``)."""
     graph = torch.is_grad_enabled()
     with torch.enable_grad():
         x = logits.view_as(logits)
@@ -160,19 +151,22 @@ class _TokenLogprobs(torch.autograd.Function):
         top_k, temperature, ignore_index = ctx.meta
         if d_logprobs is None and d_entropy is None and d_top is None:
             return None, None, None, None, None
-        if torch.is_grad_enabled() or not plain(d_logprobs, d_entropy, d_top):
+        small = [None if t is None else t.contiguous() for t in (tokens, ids, d_logprobs, d_entropy, d_top)]
+        try:
+            at = None if torch.is_grad_enabled() else [_lib.ptr(t) for t in small]
+        except RuntimeError:                # (checks beforehand would cost 4 us of the 100 us that a small call takes)
+            at = None
+        if at is None:
             grad = statement_gradient(
                 logits, lambda x: token_logprobs_reference(x, tokens, top_k, temperature, ignore_index)[:3],
                 (d_logprobs, d_entropy, d_top))
             return grad, None, None, None, None
         x, inner, ld_inner, ld_outer = logit_rows(logits)
         V = x.size(-1)
-        small = [None if t is None else t.contiguous() for t in (tokens, ids, d_logprobs, d_entropy, d_top)]
         grad = torch.empty_like(x, memory_format=torch.contiguous_format)
         rc = _lib.cuda_lib().lme_token_logprobs_bwd(
-            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // V, inner, ld_inner, ld_outer, V, _lib.ptr(small[0]),
-            ignore_index, temperature, top_k, ctx.stats.data_ptr(), *[_lib.ptr(t) for t in small[1:]],
-            grad.data_ptr(), _lib.stream_ptr())
+            x.data_ptr(), KERNEL_TYPES[x.dtype], x.numel() // V, inner, ld_inner, ld_outer, V, at[0],
+            ignore_index, temperature, top_k, ctx.stats.data_ptr(), *at[1:], grad.data_ptr(), _lib.stream_ptr())
         if rc:
             _lib.check(rc, "lme_token_logprobs_bwd")
         _lib.count_launch()
