@@ -4,15 +4,22 @@
 // With y = x / temperature, m the row's largest logit and t_j = (x_j - m) / temperature, everything that a row needs is
 //   S = sum exp(t_j),   W = sum exp(t_j) t_j,   log p_j = t_j - log S,   entropy = log S - W / S
 // and a handful of single logits.  The exponent is a difference taken in one rounding or before the product, so no large
-// numbers meet in it, whatever the temperature; sums run in fp32 per thread and are joined in 64 bits, where the few values
-// per row are finished too.
+// numbers meet in it, whatever the temperature; sums run in fp32 per thread and over the lanes of a warp, warps and CTAs are
+// joined in 64 bits, where the few values per row are finished too.
+// Fewer bits on purpose: an exponential is the hardware's 2^t (2^-22 off) of an exponent in fp32, since the exponential unit is
+// what binds a stream next (75 % busy), and what goes from a forward to its backward kernel is fp32.  Rows that a few tokens
+// dominate show it in their entropies, because those tokens' terms are not exactly one (the base follows the largest logit at a
+// distance, see Running).  Entropies relative to 64 bits, root mean square and worst, next to elementary fp32 operations that take
+// the largest logit away first: 300 single rows of 128256 bf16 logits at temperature 0.7 8e-7 and 5e-6 (3e-7, 1.4e-6), 24 rows of
+// 50257 fp32 logits 9e-8 and 7e-7 (1.1e-7, 3e-7), 333 rows of 32000 bf16 logits 2.2e-7 and 1.6e-6 (1.1e-7, 5e-7); log probabilities
+// absolutely 3.3e-7, 2.1e-7 and 2.4e-7 (5.8e-7, 2.7e-7, 2.3e-7).  Joining a warp's lanes in 64 bits too changes none of these.
 //
 // Bound by HBM (one read of the logits forward, a read and a write backward) and, sustained, by the power that the
 // instructions per logit take: a CTA of 128 threads streams a row through rings of bulk copies, one per warp; rows are split
 // over a cluster of up to 8 CTAs when there are few of them, and joined through distributed shared memory: one launch, no
 // workspace, a fixed order of sums.
-// Measured on a B200 (1000 W, sustained; up to 12 % more or less on others): scores of 4094 x 128256 bf16 logits 182 us
-// = 5.8 TB/s, with the best 64 of 4096 rows 237 us = 4.4 TB/s; gradient at 4096 x 128256 328 us = 6.4 TB/s;
+// Measured on a B200 (1000 W, sustained; up to 12 % more or less on others): scores of 4094 x 128256 bf16 logits 184 us
+// = 5.7 TB/s, with the best 64 of 4096 rows 238 us = 4.4 TB/s; gradient at 4096 x 128256 328 us = 6.4 TB/s;
 // distillation at 8192 x 128256 with the best 64, forward 344 us = 6.1 TB/s, backward 644 us = 6.5 TB/s.
 // Included by lme_cuda.cu after decode_attention.cu.
 #include <cuda_fp16.h>
@@ -249,8 +256,8 @@ struct Slice {
 template <typename T>
 struct Ring {
     static constexpr uint32_t BYTES = WARP_STEP * 16;
-    // shared addresses of this warp's stages and barriers; these have memory of their own: written over by ordinary stores, even once
-    // they had been used for the last time, they came back over what was stored
+    // Shared addresses of this warp's stages and barriers.  These have memory of their own, which nothing else is ever put into:
+    // a barrier's words may serve another purpose only after mbarrier.inval (without it they came back over ordinary stores).
     uint32_t buf, full;
     const T* source;        // of the next request
     int steps;              // those in which this warp has vectors
@@ -829,8 +836,12 @@ __device__ __forceinline__ void find_reach(Selection& sel, const float (&largest
 
 // The k best of a slice, in order, into sel.best; returns how many the slice has.  The stream has left each thread's largest
 // value and those of its segments (`group`).  What reaches the k-th largest of the threads' values are k values at least and
-// hardly more (1.2 k for k = 64 where values come in no order), so only the segments that do are read again.  Few
-// instructions matter more than few reads: the other CTAs of the SM stream meanwhile, and a warp gets every eighth slot.
+// hardly more (where values come in no order 1.4 k for k = 64, 1.3 k for 100, 1.4 k for 128), so only the segments that do are
+// read again.  Few instructions matter more than few reads: the other CTAs of the SM stream meanwhile, and a warp gets every
+// sixth slot.
+// Slices of fewer than k threads with vectors (a warp takes 128 vectors before the next has any) have no such value: all of
+// theirs are candidates, and from 1025 on they go through select_by_passes.  4096 x 2000 bf16, best 64 (63 threads): 92 us, best 80
+// 367, best 20 31; one row of 8200 in 8 slices, best 64 or more: 72 to 80 us, best 20 14.
 template <typename T>
 __device__ __noinline__ int select_best(Selection& sel, const float* group, const T* row, int V, int rank, int splits, int k,
                                         float largest, int segment_shift) {
@@ -839,7 +850,8 @@ __device__ __noinline__ int select_best(Selection& sel, const float* group, cons
     const int tid = threadIdx.x;
     // Nearly as many as there are threads: the smallest of their largest values say little (the k-th of 128 is reached by 700
     // values for k = 128, and by more than there is room for in every twentieth row).  Odd and even segments by themselves make
-    // twice as many.
+    // twice as many.  4096 x 128256 bf16 with one value per thread and with two: best 80 224 and 210 us, 100 245 and 226, 128 3370
+    // and 240.
     float halves[2] = {largest, -INFINITY};
     if (k > THREADS / 2) {
         halves[0] = -INFINITY;
@@ -1272,7 +1284,7 @@ struct DistillPart {        // of a CTA
 template <typename T, AtOne ONE>
 __global__ void __launch_bounds__(THREADS, 6) topk_distillation_kernel(const __grid_constant__ DistillArgs p) {
     constexpr int N = Elem<T>::N;
-    extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring and its barriers, then the map
+    extern __shared__ __align__(128) uint8_t vocab_smem[];  // the ring, then the map
     uint32_t* listed = reinterpret_cast<uint32_t*>(vocab_smem + RING_BYTES);
     __shared__ float red[4 * WARPS];
     __shared__ uint64_t ring_bars[WARPS * RING_STAGES];
@@ -1577,7 +1589,7 @@ __global__ void __launch_bounds__(THREADS, 8) topk_distillation_grad_kernel(cons
     if (tid < p.k) id = p.entries[r * p.k + tid];
     const bool here = g.has(id), met = here && id == label;
     const bool taken = __syncthreads_or(met);
-    if (here) {
+    if (here) {         // (fp32, and an exponential that is off by a step or two and one more for each nat)
         const float4 top = st[1], more = st[2];
         const float d = Elem<T>::f(g.x[id]) - top.x, t = d * c, e = exp2_approx(t) * top.y;
         const float lq = p.teacher[r * p.k + tid] - more.x - more.y;
@@ -1594,9 +1606,15 @@ __global__ void __launch_bounds__(THREADS, 8) topk_distillation_grad_kernel(cons
 }
 
 // ------------------------------------------------------------------ launches
-// CTAs per row: as many as fit on the GPU at once (six per SM) for all rows, while each keeps a step of work.  Beyond that
-// they only cost: 250 x 32000 fp32 logits, distillation forward, with CTAs of eight warps: 13 us with one, 18 with two; 333 x
-// 32000 bf16, scores: 9.1 and 12.2.
+// CTAs per row: as many as fit on the GPU at once (six per SM) for all rows, while each keeps about a vector for every other thread
+// at least.  Forward kernels with two CTAs per row and with one, us:
+//                        bf16, 128256 logits      fp32, 32000 logits       bf16, 32000 logits
+//   rows                 223        333           223        333           223        333        444
+//   scores               16.4 19.9  20.0 23.0      9.8 10.8  11.8 12.1      7.9  8.1   9.7  9.1  10.7  9.7
+//   with the best 20     22.6 26.2  26.5 29.9     13.9 13.7  16.2 15.1     12.5 11.6  14.4 12.7  16.2 13.2
+//   distillation         19.6 23.3  23.6 26.5     12.0 13.1  13.9 14.3     10.6 10.4  12.2 11.3  13.5 11.9
+// Long rows gain by up to a fifth, rows of some 60 KB lose by as much where there are many of them; one bound for all is taken at
+// 444 rows, where two CTAs still fit.
 inline int splits_for(long long rows, int V, int elem) {
     const int step = THREADS * 16 / elem;
     int n = 1;
